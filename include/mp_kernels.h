@@ -271,6 +271,51 @@ MP_DECL3(inner_product_bij_bjk_bik, const void* a_data, const void* b_data, cons
 MP_DECL3(inner_product_bij_bkj_bik, const void* a_data, const void* b_data, const double alpha, void* c_data, const double beta, len_t batch, len_t m, len_t n, len_t k, StreamContext stream)
 MP_DECL3(inner_product_bji_bjk_bik, const void* a_data, const void* b_data, const double alpha, void* c_data, const double beta, len_t batch, len_t m, len_t n, len_t k, StreamContext stream)
 
+/* ---- sequences that go on from a kept state --------------------------------
+ * No counterpart in the reference.  The operators of a Mamba-2 block over prompts of several lengths and over one new token
+ * per sequence, and those of a beam search.
+ *
+ * Prompt forms: the rows of all sequences lie packed behind one another; rows starts[i] .. starts[i + 1] - 1 are sequence i
+ * (starts: int32 [nseq + 1], not falling, within [0, rows]; a sequence may be empty).  Token forms: row i is the one new
+ * token of sequence i.  The state of sequence i is row slots[i] of the state buffer (int32, NULL: row i), which has nslots
+ * rows; a sequence whose slot lies outside [0, nslots) is left alone, its rows of y and all states keep what they hold, so a
+ * batch can be padded.  No two sequences of a call have the same slot (of two that had, one or the other's results would stay).
+ * A prompt goes on from its state where resume[i] != 0 (int32) and begins with zeros elsewhere (resume NULL: everywhere);
+ * a token always goes on.  The state behind the last row replaces the one before.  starts, slots and resume are DEVICE arrays.
+ * Rows of y that belong to no sequence keep what they hold.  Prompt forms: y does not overlap the inputs. */
+
+/* launch_causal_conv1d_silu that begins with the last width - 1 inputs of each sequence.
+ * states: T [nslots, width - 1, channels], the oldest input first; w, bias as there.  Token form: y may be x. */
+MP_DECL3(causal_conv1d_silu_prompt, const void* x, len_t x_pitch, const void* w, const void* bias, void* states, const void* slots, const void* resume, const void* starts, void* y, len_t y_pitch, len_t nseq, len_t rows, len_t nslots, len_t channels, len_t width, StreamContext stream)
+MP_DECL3(causal_conv1d_silu_token, const void* x, len_t x_pitch, const void* w, const void* bias, void* states, const void* slots, void* y, len_t y_pitch, len_t rows, len_t nslots, len_t channels, len_t width, StreamContext stream)
+/* The SSD scan from the projection's raw outputs (launch_ssd_scan_raw) that begins with each sequence's state:
+ *   dt = softplus(dt_raw + dt_bias[h]),  S_t = exp(-dt_t exp(A_log[h])) S_{t-1} + dt_t x_t (x) B_t,  y_t = S_t C_t.
+ * x, y: rows of heads * headdim elements, B, C: rows of ngroups * dstate, dt_raw: rows of heads, all of T with row pitches of
+ * their own (B and C share one); dt_bias, A_log: acc [heads]; states: acc [nslots, heads, headdim, dstate].  dstate is 256
+ * at most in the prompt form.  Prompt scratch: mpSsdScanPromptScratchBytes(...) bytes owned by the caller, 16-byte aligned. */
+MP_DECL3(ssd_scan_prompt, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, const void* resume, const void* starts, void* y, len_t y_pitch, void* scratch, len_t nseq, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
+MP_DECL3(ssd_scan_token, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, void* y, len_t y_pitch, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
+MP_EXTERN_C len_t mpSsdScanPromptScratchBytes(uint32_t dtype_key, len_t nseq, len_t rows, len_t heads, len_t headdim, len_t dstate, len_t ngroups);
+/* The `picks` best continuations of each search over its beams and the vocabulary, best first:
+ *   score(i, v) = scores[i] + logits[i, v] - logsumexp(logits[i, :])
+ * logits: T [batch * beams, vocab], row pitch logits_pitch; scores: acc [batch, beams].  Inside a beam the order is that of
+ * the logits (of equal ones the lower token first), between beams that of the score, formed in r64 (the lower beam first).
+ * A beam with finished[i] != 0 (int32 [batch, beams], may be NULL) goes on with the token `eos` alone, at its score.  A beam whose
+ * score is NaN or minus infinity, or whose logits hold a NaN or plus infinity or nothing above minus infinity, has no possible
+ * continuation: its tokens rank in their order with a score of minus infinity.
+ *   next_scores: acc, parents (the beam, 0 .. beams - 1), tokens, next_finished: int32, all [batch, picks];
+ *   next_finished = finished[parent] or token == eos (may be NULL).
+ * With eos >= vocab there is no end token, finished and next_finished are not used.  next_scores may be scores, next_finished
+ * may be finished (picks = beams).  beams <= 64, picks <= 32, picks <= vocab.
+ * scratch: mpBeamSelectScratchBytes(...) bytes owned by the caller, 8-byte aligned. */
+MP_DECL3(beam_select, const void* logits, len_t logits_pitch, const void* scores, const void* finished, len_t eos, void* next_scores, void* parents, void* tokens, void* next_finished, void* scratch, len_t batch, len_t beams, len_t vocab, len_t picks, StreamContext stream)
+MP_EXTERN_C len_t mpBeamSelectScratchBytes(uint32_t dtype_key, len_t batch, len_t beams, len_t vocab, len_t picks);
+/* states[l, slots[b * beams + j], :] = states[l, slots[b * beams + parents[b, j]], :] for every layer l, search b and beam j, in
+ * place, as if all were read before any is written (slots: int32 [batch * beams], distinct, NULL: row b * beams + j;
+ * parents: int32 [batch, beams]).  states: T [layers, nslots, row].  A beam whose parent lies outside [0, beams), or whose own or
+ * parent's slot lies outside [0, nslots), keeps its state.  beams <= 64.  Bit-exact. */
+MP_DECL3(reorder_states, void* states, const void* slots, const void* parents, len_t layers, len_t batch, len_t beams, len_t nslots, len_t row, StreamContext stream)
+
 /* Status word values returned by mpGetStatus (mp_device_utils.h). */
 #define MP_STATUS_OK             0u
 #define MP_STATUS_WAIT_TIMEOUT   1u  /* a bounded mbarrier wait gave up    */

@@ -81,6 +81,13 @@ LAUNCHERS = {
     "head_scale_accumulate": [P, P, P, L, L, L, CTX],
     "cross_entropy": [P, P, D, P, P, L, L, CTX],
     "neg_exp": [P, P, L, CTX],
+    # sequences that go on from a kept state
+    "causal_conv1d_silu_prompt": [P, L, P, P, P, P, P, P, P, L, L, L, L, L, L, CTX],
+    "causal_conv1d_silu_token": [P, L, P, P, P, P, P, L, L, L, L, L, CTX],
+    "ssd_scan_prompt": [P, L, P, L, P, P, P, P, L, P, P, P, P, P, L, P, L, L, L, L, L, L, L, CTX],
+    "ssd_scan_token": [P, L, P, L, P, P, P, P, L, P, P, P, L, L, L, L, L, L, L, CTX],
+    "beam_select": [P, L, P, P, L, P, P, P, P, P, L, L, L, L, CTX],
+    "reorder_states": [P, P, P, L, L, L, L, L, CTX],
     "mse_loss_i_i": [P, P, P, P, P, L, CTX],
     "bce_loss_i_i": [P, P, P, P, P, L, CTX],
     "momentum": [P, P, P, D, D, D, D, L, CTX],
@@ -126,6 +133,8 @@ UTILS = {
     "mpSsdGateRmsnormReverseScratchBytes": (L, [L, L, L, CTX]),
     "mpSsdScanScratchBytes": (L, [L, L, L, L, L, L, L, U32]),
     "mpSsdScanGenericScratchBytes": (L, [U32, L, L, L, L, L, L, U32]),
+    "mpSsdScanPromptScratchBytes": (L, [U32, L, L, L, L, L, L]),
+    "mpBeamSelectScratchBytes": (L, [U32, L, L, L, L]),
     "launch_rmsnorm_ij_j_reverse_static_r32": (C.c_int, [P, P, P, P, D, P, P, D, L, L, CTX]),
     "launch_convert_r16_r32": (None, [P, P, D, L, CTX]),
     "launch_convert_r32_r16": (None, [P, P, L, CTX]),

@@ -143,7 +143,8 @@ const Launcher kLaunchers[] = {
     MP_ENTRY(softplus_bias_reverse), MP_ENTRY(ssd_gate), MP_ENTRY(ssd_gate_reverse), MP_ENTRY(ssd_gate_rmsnorm),
     MP_ENTRY(ssd_gate_rmsnorm_reverse), MP_ENTRY(head_scale_accumulate), MP_ENTRY(cross_entropy), MP_ENTRY(neg_exp), MP_ENTRY(mse_loss_i_i),
     MP_ENTRY(bce_loss_i_i), MP_ENTRY(momentum), MP_ENTRY(permutate), MP_ENTRY(inner_product_bij_bjk_bik), MP_ENTRY(inner_product_bij_bkj_bik),
-    MP_ENTRY(inner_product_bji_bjk_bik),
+    MP_ENTRY(inner_product_bji_bjk_bik), MP_ENTRY(causal_conv1d_silu_prompt), MP_ENTRY(causal_conv1d_silu_token), MP_ENTRY(ssd_scan_prompt),
+    MP_ENTRY(ssd_scan_token), MP_ENTRY(beam_select), MP_ENTRY(reorder_states),
 };
 
 PyObject* py_launch(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {

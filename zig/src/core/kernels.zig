@@ -361,3 +361,39 @@ pub const ssd_scan_reverse_raw = dispatch_array(opaque {}, .{
     decls.launch_ssd_scan_reverse_raw_r32,
     decls.launch_ssd_scan_reverse_raw_r64,
 });
+
+pub const causal_conv1d_silu_prompt = dispatch_array(opaque {}, .{
+    decls.launch_causal_conv1d_silu_prompt_r16,
+    decls.launch_causal_conv1d_silu_prompt_r32,
+    decls.launch_causal_conv1d_silu_prompt_r64,
+});
+
+pub const causal_conv1d_silu_token = dispatch_array(opaque {}, .{
+    decls.launch_causal_conv1d_silu_token_r16,
+    decls.launch_causal_conv1d_silu_token_r32,
+    decls.launch_causal_conv1d_silu_token_r64,
+});
+
+pub const ssd_scan_prompt = dispatch_array(opaque {}, .{
+    decls.launch_ssd_scan_prompt_r16,
+    decls.launch_ssd_scan_prompt_r32,
+    decls.launch_ssd_scan_prompt_r64,
+});
+
+pub const ssd_scan_token = dispatch_array(opaque {}, .{
+    decls.launch_ssd_scan_token_r16,
+    decls.launch_ssd_scan_token_r32,
+    decls.launch_ssd_scan_token_r64,
+});
+
+pub const beam_select = dispatch_array(opaque {}, .{
+    decls.launch_beam_select_r16,
+    decls.launch_beam_select_r32,
+    decls.launch_beam_select_r64,
+});
+
+pub const reorder_states = dispatch_array(opaque {}, .{
+    decls.launch_reorder_states_r16,
+    decls.launch_reorder_states_r32,
+    decls.launch_reorder_states_r64,
+});
