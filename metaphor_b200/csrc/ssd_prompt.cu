@@ -1,16 +1,9 @@
 // The SSD scan over packed prompts that go on from a kept state (launch_ssd_scan_prompt_*):
 //   dt = softplus(raw + dt_bias[h]),  a_t = exp(-dt_t exp(A_log[h])),  S_t = a_t S_{t-1} + dt_t x_t (x) B_t,  y_t = S_t C_t
 // per sequence and head, S_{-1} the sequence's kept state or zero, the last S kept again.
-#include "mp_sequences.cuh"
+#include "ssd_prompt.cuh"
 
 namespace {
-
-struct PromptArgs {
-  const void* x; const void* raw; const void* dt_bias; const void* A_log; const void* Bm; const void* Cm; void* states; void* y;
-  size_t xp, rp, bcp, yp;
-  Sequences q;
-  int H, P, N, G;
-};
 
 // ---------------------------------------------------------------------------
 // The recurrence, step by step.  A warp has ROWS rows p of a state, PV to a lane group of eight, each lane NV of their columns in registers, so
@@ -145,7 +138,6 @@ template <typename T>
 void ssd_scan_prompt_impl(const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* Bm,
                           const void* Cm, len_t bc_pitch, void* states, const void* slots, const void* resume, const void* starts, void* y, len_t y_pitch,
                           void* scratch, len_t nseq, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext ctx) {
-  (void)scratch;
   if (ngroups == 0 || heads % ngroups != 0) MP_FATAL("ssd_scan_prompt: heads %lu not divisible by groups %lu", heads, ngroups);
   if (x_pitch < heads * headdim || y_pitch < heads * headdim || bc_pitch < ngroups * dstate || dt_pitch < heads) MP_FATAL("ssd_scan_prompt: a row pitch is below its columns");
   if (!fits(nseq) || !fits(rows) || !fits(nslots) || !fits(heads * headdim)) MP_FATAL("ssd_scan_prompt: sequences, rows, slots and columns are counted in 31 bits");
@@ -155,14 +147,21 @@ void ssd_scan_prompt_impl(const void* x, len_t x_pitch, const void* dt_raw, len_
                Sequences{static_cast<const int*>(starts), static_cast<const int*>(slots), static_cast<const int*>(resume), static_cast<int>(nseq),
                          static_cast<long long>(rows), static_cast<long long>(nslots)},
                static_cast<int>(heads), static_cast<int>(headdim), static_cast<int>(dstate), static_cast<int>(ngroups)};
+  if constexpr (std::is_same<T, __half>::value) {
+    if (mp_ssd_prompt_chunks_take(g)) {
+      if (scratch != nullptr && !mp_aligned16(scratch)) MP_FATAL("ssd_scan_prompt: scratch must be 16-byte aligned");
+      mp_ssd_prompt_chunks(g, scratch, ctx);
+      return;
+    }
+  }
   recurrence<T>(g, ctx);
 }
 
 }  // namespace
 
 extern "C" len_t mpSsdScanPromptScratchBytes(uint32_t dtype_key, len_t nseq, len_t rows, len_t heads, len_t headdim, len_t dstate, len_t ngroups) {
-  (void)dtype_key; (void)nseq; (void)rows; (void)heads; (void)headdim; (void)dstate; (void)ngroups;
-  return 256;
+  (void)ngroups;
+  return dtype_key == MP_R16 ? static_cast<len_t>(mp_ssd_prompt_chunks_scratch(nseq, rows, heads, headdim, dstate)) : 256;
 }
 
 MP_STAMP3(ssd_scan_prompt,

@@ -76,7 +76,7 @@ def test_conv_token(mp, stream, sfx, n, channels, width, pad, off):
 class Scan:
     """One call's operands: x | B | C in the rows of one buffer, raw step sizes in those of another, columns in front of each."""
 
-    def __init__(self, r, sfx, rows, nslots, heads, headdim, dstate, groups, off=0, strong=False):
+    def __init__(self, r, sfx, rows, nslots, heads, headdim, dstate, groups, off=0, strong=False, behind=1):
         self.sfx, self.dims, self.off, self.nslots = sfx, (heads, headdim, dstate, groups), off, nslots
         inner, bc = heads * headdim, groups * dstate
         self.inner, self.bc = inner, bc
@@ -86,7 +86,7 @@ class Scan:
         self.dt_bias = np.log(np.expm1(step)).astype(ref.ACC[sfx])
         self.A_log = np.log(r.uniform(1, 16, heads)).astype(ref.ACC[sfx])
         self.states = r.standard_normal((nslots, heads, headdim, dstate)).astype(ref.ACC[sfx])
-        self.y0 = ref.storage(r, (rows, inner + 1), sfx)
+        self.y0 = ref.storage(r, (rows, inner + behind), sfx)
 
     def want(self, starts, slots, resume):
         H, P, N, G = self.dims
@@ -105,12 +105,12 @@ class Scan:
                x + (self.inner + self.bc) * size, self.xbc.shape[1], d["states"], dev(slots) if slots is not None else None)
         rows = self.xbc.shape[0]
         if starts is None:
-            run(mp, stream, "ssd_scan_token", self.sfx, *ins, d["y0"], self.inner + 1, rows, self.nslots, *self.dims)
+            run(mp, stream, "ssd_scan_token", self.sfx, *ins, d["y0"], self.y0.shape[1], rows, self.nslots, *self.dims)
         else:
             n = len(starts) - 1
             nbytes = mp.lib().mpSsdScanPromptScratchBytes(TYPES.index(self.sfx), n, rows, *self.dims)
             self.scratch = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")      # NaN wherever something is read before it is written
-            run(mp, stream, "ssd_scan_prompt", self.sfx, *ins, dev(resume) if resume is not None else None, dev(starts), d["y0"], self.inner + 1,
+            run(mp, stream, "ssd_scan_prompt", self.sfx, *ins, dev(resume) if resume is not None else None, dev(starts), d["y0"], self.y0.shape[1],
                 self.scratch if scratch else None, n, rows, self.nslots, *self.dims)
         return host(d["y0"]), host(d["states"])
 
@@ -121,7 +121,7 @@ class Scan:
         mine, used = np.zeros(rows, bool), np.zeros(self.nslots, bool)
         for lo, hi, slot, _ in ref.sequences(starts, slots, resume, self.nslots):
             mine[lo:hi], used[slot] = True, True
-        assert np.array_equal(y[~mine], self.y0[~mine]) and np.array_equal(y[:, self.inner], self.y0[:, self.inner]), "rows of no sequence, or columns behind"
+        assert np.array_equal(y[~mine], self.y0[~mine]) and np.array_equal(y[:, self.inner:], self.y0[:, self.inner:]), "rows of no sequence, or columns behind"
         assert np.array_equal(states[~used], self.states[~used]), "states of no sequence"
         y = y[:, :self.inner].reshape(rows, H, P)
         within(y[mine], wy[mine], ref.scan_tolerance(self.sfx, wy, ysize, ysteps, N, True)[mine], "y")
@@ -205,6 +205,93 @@ def test_nan_stays_with_its_sequence(mp, stream, sfx):
     assert np.array_equal(y[:40], clean[0][:40]) and np.array_equal(states[slots[0]], clean[1][slots[0]])
     within(y[40:60].astype(np.float64), clean[0][40:60].astype(np.float64), np.abs(clean[0][40:60].astype(np.float64)) * 2 * ref.U_OUT[sfx] + 1e-5, "before the NaN")
     assert np.isnan(y[60:90, 5].astype(np.float64)).all() and not np.isfinite(states[slots[2]].astype(np.float64)).any()
+
+
+# Prompts in r16 whose rows are aligned: chunks on the tensor cores.
+def chunked(r, lens, shape, nslots=None, first=0, **more):
+    nslots = nslots or len(lens) + 1
+    starts, slots, resume, rows = ref.packed(r, lens, nslots, first=first)
+    return Scan(r, "r16", rows, nslots, *shape, behind=8, **more), starts, slots, resume
+
+
+@pytest.mark.parametrize("lens", [[1], [128], [2, 0, 3, 1], [127, 129, 128, 1, 0, 255, 256, 257], [3] * 60 + [0] * 3 + [140]])
+@pytest.mark.parametrize("shape", [(2, 64, 128, 1), (4, 64, 128, 2), (3, 8, 8, 3), (2, 16, 16, 2), (1, 80, 64, 1), (1, 128, 128, 1), (6, 32, 96, 3), (1, 200, 24, 1)])
+def test_chunks(mp, stream, lens, shape):
+    r = np.random.default_rng(sum(shape) + sum(lens))
+    s, starts, slots, resume = chunked(r, lens, shape, first=3)
+    if len(lens) > 3:
+        slots[2] = -1
+    s.check(s.go(mp, stream, slots, resume, starts), starts, slots, resume)
+
+
+@pytest.mark.parametrize("lens", [[700], [1000, 5, 0, 600], [256] * 3, [257, 511, 513], [0, 0, 1290]])
+@pytest.mark.parametrize("scratch", [True, False])
+def test_chunks_in_ranges(mp, stream, lens, scratch):
+    """Few sequences: cut into ranges where there is scratch, whole otherwise."""
+    r = np.random.default_rng(sum(lens))
+    s, starts, slots, resume = chunked(r, lens, (3, 64, 128, 1), first=1)
+    s.check(s.go(mp, stream, slots, resume, starts, scratch), starts, slots, resume)
+
+
+def test_chunks_in_ranges_of_partial_tiles(mp, stream):
+    r = np.random.default_rng(77)
+    s, starts, slots, resume = chunked(r, [900, 333], (2, 80, 40, 2))
+    s.check(s.go(mp, stream, slots, resume, starts), starts, slots, resume)
+
+
+@pytest.mark.parametrize("lens", [[150], [90, 7, 200], [900]])
+def test_chunks_strong_decay(mp, stream, lens):
+    r = np.random.default_rng(sum(lens))
+    s, starts, slots, resume = chunked(r, lens, (4, 64, 128, 1), strong=True)
+    s.check(s.go(mp, stream, slots, resume, starts), starts, slots, resume)
+
+
+@pytest.mark.parametrize("xs,bs,ss", [(1e-3, 1.0, 1.0), (30.0, 1.0, 1e2), (1.0, 30.0, 0.0), (1e-4, 1e-3, 1e-8), (0.0, 1.0, 1.0)])
+def test_chunks_of_any_magnitude(mp, stream, xs, bs, ss):
+    r = np.random.default_rng(31)
+    s, starts, slots, resume = chunked(r, [200, 90], (2, 64, 128, 1))
+    s.xbc[:, :s.inner] = (s.xbc[:, :s.inner].astype(np.float32) * xs).astype(np.float16)
+    s.xbc[:, s.inner:s.inner + s.bc] = (s.xbc[:, s.inner:s.inner + s.bc].astype(np.float32) * bs).astype(np.float16)
+    s.states *= np.float32(ss)
+    if xs == 1e-4:      # x and B are r16 subnormal values: their products are exact all the same
+        s.xbc[5] = np.float16(6e-8)
+    s.check(s.go(mp, stream, slots, resume, starts), starts, slots, resume)
+
+
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("what", ["x", "B", "C", "raw", "state", "neighbour"])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_chunks_with_an_infinity(mp, stream, long, what, value):
+    """What is not finite goes where the recurrence takes it, and nowhere else."""
+    r = np.random.default_rng(40)
+    lens = [700, 30] if long else [150, 130, 30]
+    s, starts, slots, resume = chunked(r, lens, (2, 64, 128, 1))
+    resume[:] = 1
+    at = starts[1] + (20 if what == "neighbour" else -57)
+    if what in ("x", "neighbour"):
+        s.xbc[at, 5] = value
+    elif what == "B":
+        s.xbc[at, s.inner + 9] = value
+    elif what == "C":
+        s.xbc[at, s.inner + s.bc + 9] = value
+    elif what == "raw":
+        s.zx[at, 3] = value
+    else:
+        s.states[slots[0], 0, 3, 7] = value
+    y, states = s.go(mp, stream, slots, resume, starts)
+    with np.errstate(all="ignore"):
+        wy, ysize, ws, ssize, ysteps, ssteps = s.want(starts, slots, resume)
+    H, P, N, G = s.dims
+    y = y[:, :s.inner].reshape(-1, H, P)
+    for got, want, size, steps, out in ((y[:starts[-1]], wy[:starts[-1]], ysize, ysteps, True), (states[slots], ws[slots], ssize, ssteps, False)):
+        got = got.astype(np.float64)
+        size, steps = (size[:starts[-1]], steps[:starts[-1]]) if out else (size[slots], steps[slots])
+        assert np.array_equal(np.isfinite(got), np.isfinite(want)) and np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+        fine = np.isfinite(want)
+        with np.errstate(all="ignore"):
+            tol = np.broadcast_to(ref.scan_tolerance("r16", want, size, steps, N, out), want.shape)
+        within(got[fine], want[fine], tol[fine], "finite part")
 
 
 # ---------------------------------------------------------------------------------------------------- selection
@@ -420,7 +507,7 @@ def test_two_streams_at_once(mp, stream):
     for s, st in zip((a, b), streams):
         x = s.d["xbc"].data_ptr()
         mp.launch("ssd_scan_prompt", torch.float16, x, s.xbc.shape[1], s.d["zx"].data_ptr() + 6, s.zx.shape[1], s.d["dt_bias"], s.d["A_log"], x + 2 * s.inner,
-                  x + 2 * (s.inner + s.bc), s.xbc.shape[1], s.d["states"], ctl[0], ctl[1], ctl[2], s.d["y0"], s.inner + 1, s.scratch, 2, rows, 2, *s.dims, st)
+                  x + 2 * (s.inner + s.bc), s.xbc.shape[1], s.d["states"], ctl[0], ctl[1], ctl[2], s.d["y0"], s.y0.shape[1], s.scratch, 2, rows, 2, *s.dims, st)
     for st in streams:
         st.sync()
         st.close()
