@@ -25,13 +25,30 @@ constexpr int CK_THREADS = 256;
 constexpr int CK_HALF = CQ * 128;               // [128 rows][128 bytes], 128-byte swizzle
 constexpr int CK_C = 0, CK_B = 2 * CK_HALF, CK_X = 4 * CK_HALF, CK_T = 5 * CK_HALF, CK_TAIL = 7 * CK_HALF;
 struct ChunkTail {
-  float colf[CQ];            // dt_j exp(l_end - l_j), l the sums inside a piece of eight steps
-  float piece[CQ / 8];       // exp(sum over the piece)
-  uint32_t most[4][8];       // per warp: largest |G|, |V|, |S|, dt as bits
-  uint64_t bar[3];
+  float piece[CQ / 8];       // decay over each piece of eight steps
+  uint32_t most[4][8];       // per warp: largest |G|, |x|, |S|, dt as bits
+  uint64_t bar[4];
   uint32_t tmem;
   int abort;
+  // What a CTA needs now and then: kept here, not in registers, of which there are none to spare (a spilled value comes back from the L2, 500
+  // cycles away: the L1 beside this much shared memory holds no thread's stack).
+  const __half *x, *B, *C, *raw;      // at the span's first row
+  __half* y;
+  float* state;                       // where the last state goes, NULL for ranges that are not a sequence's last
+  float bias, rate;
+  float plain_dt, plain_y[CP];
+  float y_down;                       // the last chunk's results over their scale in TMEM
 };
+// Weights of a chunk.  They lie over C once its products are done.
+struct ChunkWeights {
+  float diag[CQ][8];         // row i: dt_j exp(cum_i - cum_j) over its own piece, zero behind i
+  float far[CQ / 32][CQ];    // [q][j]: dt_j exp(cum - cum_j), cum up to step 32 q, for j < 32 q
+  float enter[CQ];           // decay from the beginning of the row's piece
+  float before[CQ];          // decay from the beginning of the chunk
+  float v[CQ];               // dt_j exp(E - cum_j)
+  float colf[CQ];            // dt_j times the decay towards the end of its piece
+};
+static_assert(sizeof(ChunkWeights) <= 2 * CK_HALF, "it lies over C");
 constexpr int CK_SMEM = CK_TAIL + 1024;
 static_assert(sizeof(ChunkTail) <= 1024, "two CTAs on an SM have 113 KB each");
 constexpr uint32_t TM_G = 0, TM_Y0 = 128, TM_Y1 = 192, TM_COLS = 256;
@@ -41,7 +58,8 @@ __device__ __forceinline__ void ck_cp_async(uint32_t dst, const void* src, bool 
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void ck_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void ck_cp_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+template <int GROUPS>
+__device__ __forceinline__ void ck_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(GROUPS) : "memory"); }
 __device__ __forceinline__ uint4 ck_ld(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
@@ -50,23 +68,72 @@ __device__ __forceinline__ uint4 ck_ld(uint32_t at) {
 __device__ __forceinline__ void ck_st(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+// Two fp32 values at a time.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pk(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 upk(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 both(float a) { return pk(a, a); }
 __device__ __forceinline__ float2 ck_f2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ f2 ck_wide(uint32_t v) {
+  const float2 f = ck_f2(v);
+  return pk(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t ck_narrow(f2 v) {
+  const float2 f = upk(v);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 // Two values as r16 terms: the rounded values and the rounded rest.
-__device__ __forceinline__ void ck_split(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+__device__ __forceinline__ void ck_split(f2 v, uint32_t& hi, uint32_t& lo) {
+  hi = ck_narrow(v);
+  lo = ck_narrow(fma2(ck_wide(hi), both(-1.f), v));
+}
+// Largest magnitude, NaN above all.
+__device__ __forceinline__ float most_abs(float m, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+  return r;
 }
 // The power of two that takes the largest value (its bits) to [2^13, 2^14), and its inverse.
 struct Scale { float up, down; };
-__device__ __forceinline__ Scale ck_scale(uint32_t most) {
+__device__ __forceinline__ Scale ck_scale(uint32_t most, int largest = 120) {
   int k = most == 0 ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
-  k = k > 120 ? 120 : k < -120 ? -120 : k;
+  k = k > largest ? largest : k < -120 ? -120 : k;
   return {__int_as_float((127 + k) << 23), __int_as_float((127 - k) << 23)};
 }
 __device__ __forceinline__ bool ck_infinite(uint32_t bits) { return bits >= 0x7f800000u; }
+
+// The products are a few hundred nanoseconds away: look for a while before the bounded wait, whose suspended warps wake up late.
+__device__ __forceinline__ void ck_wait(uint64_t* bar, uint32_t parity, uint32_t* status, volatile int* abort) {
+#pragma unroll 1
+  for (int i = 0; i < 4096; ++i) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(mp_smem_u32(bar)), "r"(parity)
+                 : "memory");
+    if (done) return;
+  }
+  (void)mbar_wait_abortable(bar, parity, status, abort);
+}
 
 struct ChunkArgs {
   PromptArgs g;
@@ -105,40 +172,56 @@ __device__ __forceinline__ Span span_of(const ChunkArgs& a, int id) {
   return r;
 }
 
+// A value that the compiler takes for a new one, so that what is made of it is made here and not kept in registers across the loop.
+__device__ __forceinline__ uint32_t fresh(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
 // What the two walks share: a thread's row (step, or state column n) and half of the 64 rows p; the fetch of a chunk; its step sizes.
 struct Lane { int warp, lane, row, half; };
 __device__ __forceinline__ Lane lane_of() {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (the shuffle tells the compiler that a warp takes one way: otherwise every shuffle behind a branch on it gathers the warp first)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   return {warp, lane, (warp & 3) * 32 + lane, warp >> 2};
 }
-// 128 rows of `cols` r16 values into halves of 64 columns; rows past `rows` and columns past `cols` become zeros.
+// 128 rows of `cols` r16 values into halves of 64 columns; rows past `rows` and columns past `cols` become zeros.  A thread has one 16-byte
+// column of every 32nd (one half) or 16th row, at the same place of the swizzle.
 template <int HALVES>
 __device__ __forceinline__ void fetch_tile(uint32_t dst, const __half* src, size_t pitch, int rows, int cols) {
+  constexpr int STEP = CK_THREADS / (8 * HALVES);
+  const int r = threadIdx.x / (8 * HALVES), c = threadIdx.x % (8 * HALVES);
+  const __half* from = src + r * pitch + c * 8;
+  const uint32_t to = dst + (c >> 3) * CK_HALF + ck_at(r, c & 7);
+  const int left = c * 8 < cols ? rows - r : 0;
 #pragma unroll
-  for (int k = 0; k < CQ * 8 * HALVES / CK_THREADS; ++k) {
-    const int i = k * CK_THREADS + threadIdx.x, r = i / (8 * HALVES), c = i % (8 * HALVES);
-    const bool in = r < rows && c * 8 < cols;
-    ck_cp_async(dst + (c >> 3) * CK_HALF + ck_at(r, c & 7), in ? src + r * pitch + c * 8 : src, in);
+  for (int k = 0; k < CQ / STEP; ++k) {
+    const bool in = k * STEP < left;
+    ck_cp_async(to + k * STEP * 128, in ? from : src, in);
+    from += STEP * pitch;
   }
 }
 
-// Step sizes of a chunk.  A thread has step `row`: dt, l = sum of dt A from its piece's first step on, and the piece's sum.  r64, because their
-// differences count: behind steps of strong decay a sum has no digits left in r32 for one of weak decay.
-struct StepSizes {
-  float dt;
-  double l, end;
-  __device__ __forceinline__ float behind() const { return expf(static_cast<float>(end - l)); }      // decay from this step to the end of its piece
-};
+// Step sizes of a chunk.  A thread has step `row`: dt, its decay, and the decays inside its piece of eight steps, as products of up to eight
+// factors (sums of exponents would cancel behind steps of strong decay).
+struct StepSizes { float dt, a, enter, leave, piece; };      // decay from the piece's beginning, towards its end, over all of it
 __device__ __forceinline__ StepSizes step_sizes(float raw, float bias, float rate, bool in, int lane) {
   StepSizes s;
   s.dt = in ? seq_softplus(raw + bias) : 0.f;
-  s.l = static_cast<double>(s.dt) * static_cast<double>(rate);
+  s.a = expf(s.dt * rate);
+  s.enter = s.a;
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) {
-    const double up = __shfl_up_sync(0xffffffffu, s.l, o, 8);
-    if ((lane & 7) >= o) s.l += up;
+    const float up = __shfl_up_sync(0xffffffffu, s.enter, o, 8);
+    if ((lane & 7) >= o) s.enter *= up;
   }
-  s.end = __shfl_sync(0xffffffffu, s.l, 7, 8);
+  s.leave = __shfl_down_sync(0xffffffffu, s.a, 1, 8);
+  if ((lane & 7) == 7) s.leave = 1.f;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    const float down = __shfl_down_sync(0xffffffffu, s.leave, o, 8);
+    if ((lane & 7) + o < 8) s.leave *= down;
+  }
+  s.piece = __shfl_sync(0xffffffffu, s.enter, 7, 8);
   return s;
 }
 __device__ __forceinline__ uint32_t warp_most(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
@@ -150,86 +233,99 @@ __device__ __forceinline__ uint32_t cta_most(const uint32_t* most) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// This thread's 32 values of row `row` of the x tile, and the largest of their magnitudes (NaN above all).
-__device__ __forceinline__ float load_x(uint32_t tile, const Lane& t, uint4 (&x)[4]) {
+// The largest magnitude (NaN above all) among the 32 values of the x tile that this thread fetched itself.
+__device__ __forceinline__ float most_x(uint32_t tile) {
+  constexpr int STEP = CK_THREADS / 8;
+  const uint32_t at = tile + ck_at(threadIdx.x / 8, threadIdx.x % 8);
   __half2 m = __float2half2_rn(0.f);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    x[k] = ck_ld(tile + ck_at(t.row, t.half * 4 + k));
-    const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+  for (int k = 0; k < CQ / STEP; ++k) {
+    const uint4 x = ck_ld(at + k * STEP * 128);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[e])));
   }
   const float2 f = __half22float2(m);
-  return f.x != f.x || f.y != f.y ? __int_as_float(0x7fffffff) : fmaxf(f.x, f.y);
+  return most_abs(f.x, f.y);
 }
-// V = x w in two terms, each a [128][64] tile.
-__device__ __forceinline__ void store_v(uint32_t tile, const Lane& t, const uint4 (&x)[4], float w) {
+// V = x w in two terms, each a [128][64] tile: 32 columns of a row.
+__device__ __forceinline__ void store_v(uint32_t tile, uint32_t x_tile, int row, int half, float w) {
+  const f2 w2 = both(w);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t in[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+    const uint32_t at = ck_at(row, half * 4 + k);
+    const uint4 x = ck_ld(x_tile + at);
+    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = ck_f2(in[e]);
-      ck_split(f.x * w, f.y * w, hi[e], lo[e]);
-    }
-    const uint32_t at = tile + ck_at(t.row, t.half * 4 + k);
-    ck_st(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-    ck_st(at + CK_HALF, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    for (int e = 0; e < 4; ++e) ck_split(mul2(ck_wide(in[e]), w2), hi[e], lo[e]);
+    ck_st(tile + at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+    ck_st(tile + at + CK_HALF, make_uint4(lo[0], lo[1], lo[2], lo[3]));
   }
 }
 // S in two terms the same way: this thread's row is a state column n.
-__device__ __forceinline__ void store_s(uint32_t tile, const Lane& t, const float (&S)[32], float up) {
+__device__ __forceinline__ void store_s(uint32_t tile, const Lane& t, const f2 (&S)[16], float up) {
+  const f2 up2 = both(up);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ck_split(S[k * 8 + 2 * e] * up, S[k * 8 + 2 * e + 1] * up, hi[e], lo[e]);
+    for (int e = 0; e < 4; ++e) ck_split(mul2(S[k * 4 + e], up2), hi[e], lo[e]);
     const uint32_t at = tile + ck_at(t.row, t.half * 4 + k);
     ck_st(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
     ck_st(at + CK_HALF, make_uint4(lo[0], lo[1], lo[2], lo[3]));
   }
 }
-__device__ __forceinline__ uint32_t most_of(const float (&S)[32]) {
-  uint32_t m = 0;
+__device__ __forceinline__ uint32_t most_of(const f2 (&S)[16]) {
+  float m = 0.f;
 #pragma unroll
-  for (int p = 0; p < 32; ++p) m = max(m, abs_bits(S[p]));
-  return m;
+  for (int p = 0; p < 16; ++p) {
+    const float2 v = upk(S[p]);
+    m = most_abs(most_abs(m, v.x), v.y);
+  }
+  return abs_bits(m);
+}
+// S = total S + down v, v from TMEM
+__device__ __forceinline__ void add_state(f2 (&S)[16], uint32_t tmem, float total, float down) {
+  const f2 t2 = both(total), d2 = both(down);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint32_t v[16];
+    tmem_ld_32x16(tmem + k * 16, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int p = 0; p < 8; ++p) S[8 * k + p] = fma2(t2, S[8 * k + p], mul2(d2, pk(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1]))));
+  }
 }
 
-// A chunk step by step, for values that the products would spread.  The thread has S[n = row][p = 32 half ..]; y_p is summed over a warp's 32
-// columns n lane against lane, then over the four warps through shared memory.  OUT: with y.
+// A chunk step by step, for values that the products would spread.  S lies where the operands' terms were, [64 p][128 n]; a thread has column
+// n = row, 32 rows p.  y_p is summed over a warp's 32 columns lane against lane, then over the warps in turn.  OUT: with y.
 template <bool OUT>
-__device__ __noinline__ void chunk_plain_steps(unsigned char* smem, uint32_t base, const Lane t, float* state, float dt, float rate, int steps, __half* y, size_t yp,
-                                         int pcols) {
-  float* sdt = reinterpret_cast<float*>(smem + CK_T);                   // the place of the terms, which no product reads now
-  float* part = sdt + CQ;                                               // [4][64]
-  float S[32];
+__device__ __forceinline__ void chunk_plain(unsigned char* smem, ChunkTail* tail, const Lane& t, f2 (&S)[16], float dt, int steps, __half* y, size_t yp, int pcols) {
+  float* held = reinterpret_cast<float*>(smem + CK_T) + t.half * 32 * CN + t.row;
 #pragma unroll
-  for (int p = 0; p < 32; ++p) S[p] = state[p];
-  __syncthreads();
-  if (t.half == 0) sdt[t.row] = dt;
-  __syncthreads();
+  for (int p = 0; p < 16; ++p) {
+    const float2 v = upk(S[p]);
+    held[2 * p * CN] = v.x;
+    held[(2 * p + 1) * CN] = v.y;
+  }
+#pragma unroll 1
   for (int i = 0; i < steps; ++i) {
-    const float d = sdt[i], a = expf(d * rate);
+    __syncthreads();
+    if (t.half == 0 && t.row == i) tail->plain_dt = dt;
+    if (threadIdx.x < CP) tail->plain_y[threadIdx.x] = 0.f;
+    __syncthreads();
+    const float d = tail->plain_dt, a = expf(d * tail->rate);
     const uint32_t col = (t.row >> 6) * CK_HALF + ck_at(i, (t.row & 63) >> 3) + (t.row & 7) * 2;
     const float b = __half2float(*reinterpret_cast<const __half*>(smem + CK_B + col));
     const float c = OUT ? __half2float(*reinterpret_cast<const __half*>(smem + CK_C + col)) : 0.f;
     float v[32];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint4 x = ck_ld(base + CK_X + ck_at(i, t.half * 4 + k));
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = ck_f2(w[e]);
-        const int p = k * 8 + 2 * e;
-        S[p] = a * S[p] + d * f.x * b;
-        S[p + 1] = a * S[p + 1] + d * f.y * b;
-        v[p] = c * S[p];
-        v[p + 1] = c * S[p + 1];
-      }
+    for (int p = 0; p < 32; ++p) {
+      const float x = __half2float(*reinterpret_cast<const __half*>(smem + CK_X + ck_at(i, t.half * 4 + (p >> 3)) + (p & 7) * 2));
+      const float now = a * held[p * CN] + d * x * b;
+      held[p * CN] = now;
+      v[p] = c * now;
     }
     if (OUT) {
 #pragma unroll
@@ -240,26 +336,17 @@ __device__ __noinline__ void chunk_plain_steps(unsigned char* smem, uint32_t bas
           const float send = up ? v[p] : v[p + o], keep = up ? v[p + o] : v[p];
           v[p] = keep + __shfl_xor_sync(0xffffffffu, send, o);
         }
-      part[(t.warp & 3) * 64 + t.half * 32 + t.lane] = v[0];
-      __syncthreads();
-      if (threadIdx.x < CP && static_cast<int>(threadIdx.x) < pcols)
-        y[i * yp + threadIdx.x] = __float2half_rn(part[threadIdx.x] + part[64 + threadIdx.x] + part[128 + threadIdx.x] + part[192 + threadIdx.x]);
-      __syncthreads();
+#pragma unroll 1
+      for (int w = 0; w < 4; ++w) {
+        if ((t.warp & 3) == w) tail->plain_y[t.half * 32 + t.lane] += v[0];
+        __syncthreads();
+      }
+      if (static_cast<int>(threadIdx.x) < pcols) y[i * yp + threadIdx.x] = __float2half_rn(tail->plain_y[threadIdx.x]);
     }
   }
+#pragma unroll
+  for (int p = 0; p < 16; ++p) S[p] = pk(held[2 * p * CN], held[(2 * p + 1) * CN]);
   __syncthreads();
-#pragma unroll
-  for (int p = 0; p < 32; ++p) state[p] = S[p];
-}
-template <bool OUT>      // (a copy goes through memory, so that S itself stays in registers)
-__device__ __forceinline__ void chunk_plain(unsigned char* smem, uint32_t base, const Lane& t, float (&S)[32], float dt, float rate, int steps, __half* y, size_t yp,
-                                            int pcols) {
-  float copy[32];
-#pragma unroll
-  for (int p = 0; p < 32; ++p) copy[p] = S[p];
-  chunk_plain_steps<OUT>(smem, base, t, copy, dt, rate, steps, y, yp, pcols);
-#pragma unroll
-  for (int p = 0; p < 32; ++p) S[p] = copy[p];
 }
 
 // ---------------------------------------------------------------------------
@@ -268,11 +355,12 @@ __device__ __forceinline__ void chunk_plain(unsigned char* smem, uint32_t base, 
 __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkArgs a) {
   extern __shared__ __align__(1024) unsigned char ck_smem[];
   ChunkTail* tail = reinterpret_cast<ChunkTail*>(ck_smem + CK_TAIL);
+  ChunkWeights* wt = reinterpret_cast<ChunkWeights*>(ck_smem + CK_C);
   const PromptArgs& g = a.g;
   const Lane t = lane_of();
   const uint32_t base = mp_smem_u32(ck_smem);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 3; ++i) mbar_init(tail->bar + i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(tail->bar + i, 1);
     mbar_fence_init();
     tail->abort = 0;
   }
@@ -282,73 +370,107 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
   const Span sp = span_of(a, id);
   if (!sp.any) { mp_launch_dependents(); return; }
   if (t.warp == 0) tmem_alloc(&tail->tmem, TM_COLS);
-  const int pcols = min(CP, g.P - p0);
-  const __half* x = static_cast<const __half*>(g.x) + static_cast<size_t>(h) * g.P + p0;
-  const __half* raw = static_cast<const __half*>(g.raw) + h;
-  const __half* Bm = static_cast<const __half*>(g.Bm) + static_cast<size_t>(grp) * g.N;
-  const __half* Cm = static_cast<const __half*>(g.Cm) + static_cast<size_t>(grp) * g.N;
-  __half* y = static_cast<__half*>(g.y) + static_cast<size_t>(h) * g.P + p0;
+  const int pcols = min(CP, g.P - p0), length = static_cast<int>(sp.hi - sp.lo);
   float* state = static_cast<float*>(g.states) + ((sp.slot * g.H + h) * g.P + p0) * static_cast<long long>(g.N);
-  const float bias = static_cast<const float*>(g.dt_bias)[h], rate = -expf(static_cast<const float*>(g.A_log)[h]);
-
-  auto fetch = [&](long long t0, int steps) {
-    fetch_tile<2>(base + CK_C, Cm + t0 * g.bcp, g.bcp, steps, g.N);
-    fetch_tile<2>(base + CK_B, Bm + t0 * g.bcp, g.bcp, steps, g.N);
-    fetch_tile<1>(base + CK_X, x + t0 * g.xp, g.xp, steps, pcols);
+  if (threadIdx.x == 0) {
+    tail->x = static_cast<const __half*>(g.x) + sp.lo * g.xp + static_cast<size_t>(h) * g.P + p0;
+    tail->B = static_cast<const __half*>(g.Bm) + sp.lo * g.bcp + static_cast<size_t>(grp) * g.N;
+    tail->C = static_cast<const __half*>(g.Cm) + sp.lo * g.bcp + static_cast<size_t>(grp) * g.N;
+    tail->raw = static_cast<const __half*>(g.raw) + sp.lo * g.rp + h;
+    tail->y = static_cast<__half*>(g.y) + sp.lo * g.yp + static_cast<size_t>(h) * g.P + p0;
+    tail->state = sp.hi == sp.seq_hi ? state : nullptr;
+    tail->bias = static_cast<const float*>(g.dt_bias)[h];
+    tail->rate = -expf(static_cast<const float*>(g.A_log)[h]);
+  }
+  __syncthreads();
+  auto steps_at = [&](int t0) { return min(length - t0, CQ); };
+  float raw_next = 0.f;      // of the warps that make the weights
+  auto fetch_bc = [&](int t0) {
+    const int steps = steps_at(t0);
+    const uint32_t at = fresh(base);
+    fetch_tile<2>(at + CK_C, tail->C + t0 * g.bcp, g.bcp, steps, g.N);
+    fetch_tile<2>(at + CK_B, tail->B + t0 * g.bcp, g.bcp, steps, g.N);
+    ck_cp_commit();
+    if (t.half == 0) raw_next = t.row < steps ? __half2float(tail->raw[(t0 + t.row) * g.rp]) : 0.f;
+  };
+  auto fetch_x = [&](int t0) {
+    fetch_tile<1>(fresh(base) + CK_X, tail->x + t0 * g.xp, g.xp, steps_at(t0), pcols);
     ck_cp_commit();
   };
-  auto steps_at = [&](long long t0) { return sp.hi - t0 < CQ ? static_cast<int>(sp.hi - t0) : CQ; };
-  float raw_next = 0.f;
-  auto fetch_raw = [&](long long t0) { raw_next = t0 + t.row < sp.hi ? __half2float(raw[(t0 + t.row) * g.rp]) : 0.f; };
-  if (sp.lo < sp.hi) {
-    fetch(sp.lo, steps_at(sp.lo));
-    fetch_raw(sp.lo);
+  if (length > 0) {
+    fetch_bc(0);
+    fetch_x(0);
   }
   // the state that the span receives: this thread's column n = row, rows p = 32 half ..
-  float S[32];
+  f2 S[16];
   {
-    const float* from = nullptr;
+    const float* from = state;
     long long pitch = g.N;
+    bool any = true;
     if (a.range != 0 && sp.lo > sp.seq_lo) {
       from = a.local + (static_cast<size_t>(id) * units + unit) * CP * CN;
       pitch = CN;
-    } else if (seq_resumes(g.q, sp.s)) {
-      from = state;
+    } else {
+      any = seq_resumes(g.q, sp.s);
     }
+    const int live = any && t.row < g.N ? pcols - t.half * 32 : 0;
+    from += t.half * 32 * pitch + t.row;
 #pragma unroll
-    for (int p = 0; p < 32; ++p) S[p] = from != nullptr && t.row < g.N && t.half * 32 + p < pcols ? from[(t.half * 32 + p) * pitch + t.row] : 0.f;
+    for (int p = 0; p < 16; ++p) {
+      float v0 = 0.f, v1 = 0.f;
+      if (2 * p < live) v0 = *from;
+      from += pitch;
+      if (2 * p + 1 < live) v1 = *from;
+      from += pitch;
+      S[p] = pk(v0, v1);
+    }
   }
   auto publish = [&]() {      // S becomes an operand of the next chunk: its terms under one power of two
     const uint32_t m = warp_most(most_of(S));
     if (t.lane == 0) tail->most[2][t.warp] = m;
     __syncthreads();
     const uint32_t most = cta_most(tail->most[2]);
-    if (!ck_infinite(most)) store_s(base + CK_T, t, S, ck_scale(most).up);
+    if (!ck_infinite(most)) store_s(fresh(base) + CK_T, t, S, ck_scale(most).up);
     return most;
   };
   uint32_t s_most = publish();
 
-  const uint64_t d_c = umma_smem_desc(base + CK_C, 16, 1024), d_b = umma_smem_desc(base + CK_B, 16, 1024), d_bt = umma_smem_desc(base + CK_B, CK_HALF, 1024);
-  const uint64_t d_x = umma_smem_desc(base + CK_X, CK_HALF, 1024), d_t = umma_smem_desc(base + CK_T, CK_HALF, 1024);
   constexpr uint32_t id_g = umma_instr_desc(UMMA_FMT_F16, 0, 0, 128, 128), id_y = umma_instr_desc(UMMA_FMT_F16, 0, 1, 128, CP), id_s = umma_instr_desc(UMMA_FMT_F16, 1, 1, 128, CP);
   constexpr uint32_t HALF_U = CK_HALF / 16, ROWS_U = 16 * 128 / 16;
   auto kslice = [](int ks) { return static_cast<uint32_t>((ks >> 2) * HALF_U + (ks & 3) * 2); };
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
-  const uint32_t tmem = tail->tmem, tq = tmem + (static_cast<uint32_t>(t.warp & 3) << 21);      // this warp's 32 lanes
+  auto lanes = [&]() { return tail->tmem + (static_cast<uint32_t>(t.warp & 3) << 21); };      // this warp's 32 lanes of TMEM
   uint32_t issued = 0, finished = 0;      // phases of the barriers: scores and C S^T, the other two products
-  const bool odd = !(fabsf(rate) < INFINITY);
-  for (long long t0 = sp.lo; t0 < sp.hi; t0 += CQ) {
+  // The results of a chunk leave TMEM while the next one's first products run.
+  bool pending = false;
+  auto store_y = [&](int t0, int steps) {
+    const f2 down = both(tail->y_down);
+    __half* out = tail->y + (t0 + t.row) * g.yp + t.half * 32;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t v[16], o[8];
+      tmem_ld_32x16(lanes() + TM_Y1 + t.half * 32 + k * 16, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int p = 0; p < 8; ++p) o[p] = ck_narrow(mul2(pk(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1])), down));
+      if (t.row < steps && t.half * 32 + k * 16 < pcols) *reinterpret_cast<uint4*>(out + k * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+      if (t.row < steps && t.half * 32 + k * 16 + 8 < pcols) *reinterpret_cast<uint4*>(out + k * 16 + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+  };
+  for (int t0 = 0; t0 < length; t0 += CQ) {
     const int steps = steps_at(t0);
-    const bool carried = s_most != 0, products = !odd && !ck_infinite(s_most);
-    ck_cp_wait();
+    const bool carried = s_most != 0, products = !ck_infinite(s_most) && fabsf(tail->rate) < INFINITY;
+    ck_cp_wait<1>();      // C and B
     fence_proxy_async_smem();
     tcgen05_fence_before_sync();
     __syncthreads();
     if (tail->abort != 0) break;      // a wait ran out
     tcgen05_fence_after_sync();
     if (t.warp == 0 && products && elect_one()) {
+      const uint32_t at = fresh(base), tmem = tail->tmem;
+      const uint64_t d_c = umma_smem_desc(at + CK_C, 16, 1024), d_b = umma_smem_desc(at + CK_B, 16, 1024), d_t = umma_smem_desc(at + CK_T, CK_HALF, 1024);
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) umma<false>(tmem + TM_G, d_c + kslice(ks), d_b + kslice(ks), id_g, ks != 0 ? 1u : 0u);
       umma_commit(tail->bar + 0);
@@ -360,163 +482,202 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
       umma_commit(tail->bar + 1);
     }
     __syncwarp();
-    const StepSizes z = step_sizes(raw_next, bias, rate, t.row < steps, t.lane);
+    if (pending) store_y(t0 - CQ, CQ);
+    pending = false;
+    // half of the warps make the weights
+    StepSizes z;
+    float far[4], diag[8], before = 1.f;      // far: from this step's piece on to steps 32, 64, 96 and the end
     if (t.half == 0) {
-      tail->colf[t.row] = z.dt * z.behind();
-      if ((t.lane & 7) == 7) tail->piece[t.row >> 3] = expf(static_cast<float>(z.end));
+      z = step_sizes(raw_next, tail->bias, tail->rate, t.row < steps, t.lane);
+      if ((t.lane & 7) == 7) tail->piece[t.row >> 3] = z.piece;
+      const uint32_t dm = warp_most(abs_bits(z.dt));
+      if (t.lane == 0) tail->most[3][t.warp] = dm;
+      named_bar_sync(1, CK_THREADS / 2);
+      float f = z.dt * z.leave;
+#pragma unroll
+      for (int k = 0; k < CQ / 8; ++k) {
+        const float d = tail->piece[k];
+        if (k < (t.row >> 3)) before *= d;
+        if (k > (t.row >> 3)) f *= d;
+        if ((k & 3) == 3) far[k >> 2] = f;
+      }
+      float left = 1.f, au = z.a, du = z.dt;      // k steps back: the decays of the steps behind, dt
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        diag[k] = k <= (t.lane & 7) ? du * left : 0.f;
+        left *= au;
+        au = __shfl_up_sync(0xffffffffu, au, 1, 8);
+        du = __shfl_up_sync(0xffffffffu, du, 1, 8);
+      }
     }
-    uint4 xv[4];
-    const float x_most = load_x(base + CK_X, t, xv);
-    const uint32_t vm = warp_most(abs_bits(x_most * z.dt)), dm = warp_most(abs_bits(z.dt));
-    if (t.lane == 0) { tail->most[1][t.warp] = vm; tail->most[3][t.warp] = dm; }
+    ck_cp_wait<0>();      // this thread's x
+    const uint32_t xm = warp_most(abs_bits(most_x(fresh(base) + CK_X)));
+    if (t.lane == 0) tail->most[1][t.warp] = xm;
+    const int q = t.warp & 3;      // this warp's rows begin at 32 q: blocks of 16 score columns up to 2 q + 1 are below or on the diagonal; it has
+                                   // every other one
     if (products) {
-      (void)mbar_wait_abortable(tail->bar + 0, issued, a.status, &tail->abort);
+      ck_wait(tail->bar + 0, issued, a.status, &tail->abort);
       tcgen05_fence_after_sync();
-      uint32_t gm = 0;
+      float gm = 0.f;
+      const uint32_t tg = lanes() + TM_G + t.half * 16;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        uint32_t v[16];
-        tmem_ld_32x16(tq + TM_G + (2 * b + t.half) * 16, v);
-        tmem_ld_wait();
+        if (b <= q) {
+          uint32_t v[16];
+          tmem_ld_32x16(tg + b * 32, v);
+          tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) gm = max(gm, v[e] & 0x7fffffffu);
+          for (int e = 0; e < 16; ++e) gm = most_abs(gm, __uint_as_float(v[e]));
+        }
       }
-      gm = warp_most(gm);
-      if (t.lane == 0) tail->most[0][t.warp] = gm;
-      (void)mbar_wait_abortable(tail->bar + 1, issued, a.status, &tail->abort);
+      const uint32_t gw = warp_most(abs_bits(gm));
+      if (t.lane == 0) tail->most[0][t.warp] = gw;
+      ck_wait(tail->bar + 1, issued, a.status, &tail->abort);
       tcgen05_fence_after_sync();
       issued ^= 1;
+      if (t.half == 0) {      // C is free
+        wt->enter[t.row] = z.enter;
+        wt->before[t.row] = before * z.enter;
+        wt->colf[t.row] = z.dt * z.leave;
+        wt->v[t.row] = far[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) wt->far[k + 1][t.row] = far[k];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) wt->diag[t.row][(t.lane - k) & 7] = diag[k];
+      }
     }
     __syncthreads();
-    // bounds of V and W: the weights that are left out of them are at most one
-    const uint32_t v_most = cta_most(tail->most[1]);
-    const uint32_t w_most = products ? abs_bits(__uint_as_float(cta_most(tail->most[0])) * __uint_as_float(cta_most(tail->most[3]))) : 0u;
-    float after = 1.f, total = 1.f, before = 1.f;      // decay behind this thread's piece, of the chunk, and up to this step
-#pragma unroll
-    for (int k = 0; k < CQ / 8; ++k) {
-      const float d = tail->piece[k];
-      total *= d;
-      if (k > (t.row >> 3)) after *= d;
-      if (k < (t.row >> 3)) before *= d;
-    }
-    before *= expf(static_cast<float>(z.l));
+    // bounds of V and W: the decays that are left out of them are at most one
+    const float dt_most = __uint_as_float(max(max(tail->most[3][0], tail->most[3][1]), max(tail->most[3][2], tail->most[3][3])));
+    const uint32_t v_most = abs_bits(__uint_as_float(cta_most(tail->most[1])) * dt_most);
+    const uint32_t w_most = products ? abs_bits(__uint_as_float(cta_most(tail->most[0])) * dt_most) : 0u;
     if (!products || ck_infinite(v_most) || ck_infinite(w_most)) {
-      chunk_plain<true>(ck_smem, base, t, S, z.dt, rate, steps, y + t0 * g.yp, g.yp, pcols);
+      if (products) {      // the weights lie over C
+        __syncthreads();
+        fetch_tile<2>(base + CK_C, tail->C + t0 * g.bcp, g.bcp, steps, g.N);
+        ck_cp_commit();
+        ck_cp_wait<0>();
+      }
+      chunk_plain<true>(ck_smem, tail, t, S, z.dt, steps, tail->y + t0 * g.yp, g.yp, pcols);
     } else {
-      const Scale sv = ck_scale(v_most), sw = ck_scale(w_most);
-      store_v(base + CK_T, t, xv, z.dt * z.behind() * after * sv.up);
-      float y0[32];
-      if (carried) {
-        tmem_ld_32x32(tq + TM_Y0 + t.half * 32, reinterpret_cast<uint32_t*>(y0));
-        tmem_ld_wait();
-        const float f = before * ck_scale(s_most).down;
-#pragma unroll
-        for (int p = 0; p < 32; ++p) y0[p] *= f;
-      } else {
-#pragma unroll
-        for (int p = 0; p < 32; ++p) y0[p] = 0.f;
+      // (2^60: scores below 2^-47 do not show in y, and the state's share, which takes the same scale, stays finite)
+      const Scale sv = ck_scale(v_most), sw = ck_scale(w_most, 60);
+      const uint32_t tiles = fresh(base);
+      // V goes to the warps with few blocks of W: four pieces of 32 rows and 32 columns to the first two, two each to the next
+      for (int u = q == 0 ? 2 * t.half : 2 * q + 2 + t.half, n = q == 0 ? 2 : q == 3 ? 0 : 1; n > 0; ++u, --n) {
+        const int row = (u >> 1) * 32 + t.lane;
+        store_v(tiles + CK_T, tiles + CK_X, row, u & 1, wt->v[row] * sv.up);
       }
-      // W over G: sixteen columns of scores become eight of the upper terms and eight of the lower ones
-      float diag[8];      // this row's weights inside its own piece
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double lj = __shfl_sync(0xffffffffu, z.l, e, 8);
-        const float dj = __shfl_sync(0xffffffffu, z.dt, e, 8);
-        diag[e] = e <= (t.lane & 7) ? dj * expf(static_cast<float>(z.l - lj)) * sw.up : 0.f;
-      }
-      const int mine = t.row >> 3;
-      const float enter = expf(static_cast<float>(z.l)) * sw.up;      // towards the end of the piece before
-      float far = 0.f;
+      {
+        // W over G: sixteen columns of scores become eight of the upper terms and eight of the lower ones
+        const float4 P = *reinterpret_cast<const float4*>(tail->piece + 4 * q);
+        const int r = t.lane >> 3;      // this row's piece among the four of its warp
+        const float enter = wt->enter[t.row] * sw.up;
+        const float p1 = r > 1 ? P.y : 1.f, p2 = r > 2 ? P.z : 1.f;
+        const f2 lead = both(enter * (r > 0 ? P.x : 1.f) * p1 * p2), up = both(sw.up);
+        const uint32_t tg = lanes() + TM_G + t.half * 16;
+        uint32_t v[16];
+        tmem_ld_32x16(tg, v);
 #pragma unroll 1
-      for (int blk = 7; blk >= 0; --blk) {
-        const bool here = (blk & 1) == t.half, none = blk > 2 * (t.warp & 3) + 1;
-        uint32_t v[16], w[16];
-        if (here && !none) {
-          tmem_ld_32x16(tq + TM_G + blk * 16, v);
-          tmem_ld_wait();
-        }
+        for (int b = 0; b < 4; ++b) {
+          uint32_t w[16];
+          if (b <= q) {
+            tmem_ld_wait();
+            const float4* cf = reinterpret_cast<const float4*>((b < q ? wt->far[q] : wt->colf) + b * 32 + t.half * 16);
 #pragma unroll
-        for (int hp = 1; hp >= 0; --hp) {
-          const int piece = 2 * blk + hp;
-          if (mine == piece + 1) far = enter;
-          if (here && !none) {
-            const float4 c0 = *reinterpret_cast<const float4*>(tail->colf + piece * 8), c1 = *reinterpret_cast<const float4*>(tail->colf + piece * 8 + 4);
-            const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            for (int k = 0; k < 2; ++k) {      // a piece of eight columns
+              // Below the warp's own 32 columns one factor for a row; there, two pieces for each half: those before the row's own, its own, zeros behind
+              const int piece = 2 * t.half + k;
+              const bool own = b == q && r == piece;
+              const f2 row = b < q ? lead : own ? up : r > piece ? both(t.half == 0 ? (k == 0 ? enter * p1 * p2 : enter * p2) : enter) : both(0.f);
+              const float4* from = own ? reinterpret_cast<const float4*>(wt->diag[t.row]) : cf + 2 * k;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float w0 = mine == piece ? diag[2 * e] : far * c[2 * e], w1 = mine == piece ? diag[2 * e + 1] : far * c[2 * e + 1];
-              ck_split(__uint_as_float(v[hp * 8 + 2 * e]) * w0, __uint_as_float(v[hp * 8 + 2 * e + 1]) * w1, w[hp * 4 + e], w[8 + hp * 4 + e]);
+              for (int e = 0; e < 2; ++e) {
+                const float4 c = from[e];
+                const int at = 8 * k + 4 * e;
+                ck_split(mul2(pk(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), mul2(row, pk(c.x, c.y))), w[4 * k + 2 * e], w[8 + 4 * k + 2 * e]);
+                ck_split(mul2(pk(__uint_as_float(v[at + 2]), __uint_as_float(v[at + 3])), mul2(row, pk(c.z, c.w))), w[4 * k + 2 * e + 1], w[8 + 4 * k + 2 * e + 1]);
+              }
             }
-          }
-          far *= tail->piece[piece];
-        }
-        if (here) {
-          if (none) {
+            if (b < q) tmem_ld_32x16(tg + (b + 1) * 32, v);
+          } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = 0;
           }
-          tmem_st_32x16(tq + TM_G + blk * 16, w);
+          tmem_st_32x16(tg + b * 32, w);
         }
       }
+      if (carried) {      // the state's share of y, to the scale of W: W x is added to it
+        const f2 f = both(wt->before[t.row] * ck_scale(cta_most(tail->most[2])).down * sw.up);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t v[16];
+          tmem_ld_32x16(lanes() + TM_Y0 + t.half * 32 + k * 16, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            const float2 r = upk(mul2(f, pk(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1]))));
+            v[2 * p] = __float_as_uint(r.x);
+            v[2 * p + 1] = __float_as_uint(r.y);
+          }
+          tmem_st_32x16(lanes() + TM_Y1 + t.half * 32 + k * 16, v);
+        }
+      }
+      if (threadIdx.x == 0) tail->y_down = sw.down;
       tmem_st_wait();
       fence_proxy_async_smem();
       tcgen05_fence_before_sync();
       __syncthreads();
       tcgen05_fence_after_sync();
       if (t.warp == 0 && elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < 16; ++ks)
-          umma_f16_ta(tmem + TM_Y1, tmem + TM_G + (ks & 7) * 16 + (ks >> 3) * 8, d_x + (ks & 7) * ROWS_U, id_y, ks != 0 ? 1u : 0u);
+        const uint32_t at = fresh(base), tmem = tail->tmem;
+        const uint64_t d_bt = umma_smem_desc(at + CK_B, CK_HALF, 1024), d_t = umma_smem_desc(at + CK_T, CK_HALF, 1024), d_x = umma_smem_desc(at + CK_X, CK_HALF, 1024);
 #pragma unroll
         for (int ks = 0; ks < 16; ++ks)
           umma<false>(tmem + TM_Y0, d_bt + (ks & 7) * ROWS_U, d_t + (ks >> 3) * HALF_U + (ks & 7) * ROWS_U, id_s, ks != 0 ? 1u : 0u);
         umma_commit(tail->bar + 2);
+#pragma unroll
+        for (int ks = 0; ks < 16; ++ks)
+          umma_f16_ta(tmem + TM_Y1, tmem + TM_G + (ks & 7) * 16 + (ks >> 3) * 8, d_x + (ks & 7) * ROWS_U, id_y, ks != 0 || carried ? 1u : 0u);
+        umma_commit(tail->bar + 3);
       }
       __syncwarp();
-      (void)mbar_wait_abortable(tail->bar + 2, finished, a.status, &tail->abort);
-      finished ^= 1;
+      pending = true;
+      ck_wait(tail->bar + 2, finished, a.status, &tail->abort);
       tcgen05_fence_after_sync();
-      {
-        float v[32];
-        tmem_ld_32x32(tq + TM_Y1 + t.half * 32, reinterpret_cast<uint32_t*>(v));
-        tmem_ld_wait();
-        if (t.row < steps) {
-          __half* out = y + (t0 + t.row) * g.yp + t.half * 32;
+      if (t0 + CQ < length) fetch_bc(t0 + CQ);
+      float total = 1.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int p = k * 8 + 2 * e;
-              const __half2 hv = __floats2half2_rn(y0[p] + v[p] * sw.down, y0[p + 1] + v[p + 1] * sw.down);
-              o[e] = *reinterpret_cast<const uint32_t*>(&hv);
-            }
-            if (t.half * 32 + k * 8 < pcols) *reinterpret_cast<uint4*>(out + k * 8) = make_uint4(o[0], o[1], o[2], o[3]);
-          }
-        }
-        tmem_ld_32x32(tq + TM_Y0 + t.half * 32, reinterpret_cast<uint32_t*>(v));
-        tmem_ld_wait();
-#pragma unroll
-        for (int p = 0; p < 32; ++p) S[p] = total * S[p] + v[p] * sv.down;
-      }
+      for (int k = 0; k < CQ / 8; ++k) total *= tail->piece[k];
+      add_state(S, lanes() + TM_Y0 + t.half * 32, total, sv.down);
+      tcgen05_fence_before_sync();
     }
-    if (t0 + CQ < sp.hi) {
-      __syncthreads();      // plain: every thread has read the tiles
-      fetch(t0 + CQ, steps_at(t0 + CQ));
-      fetch_raw(t0 + CQ);
+    if (t0 + CQ < length) {
+      if (!pending) fetch_bc(t0 + CQ);
       s_most = publish();
     }
+    if (pending) {
+      ck_wait(tail->bar + 3, finished, a.status, &tail->abort);
+      tcgen05_fence_after_sync();
+      finished ^= 1;
+    }
+    if (t0 + CQ < length) fetch_x(t0 + CQ);
   }
+  if (pending) store_y((length - 1) / CQ * CQ, (length - 1) % CQ + 1);
   mp_launch_dependents();
-  if (sp.hi == sp.seq_hi && t.row < g.N) {
+  state = tail->state;
+  if (state != nullptr && t.row < g.N) {
 #pragma unroll
     for (int p = 0; p < 32; ++p)
-      if (t.half * 32 + p < pcols) state[(t.half * 32 + p) * static_cast<long long>(g.N) + t.row] = S[p];
+      if (t.half * 32 + p < pcols) {
+        const float2 v = upk(S[p / 2]);
+        state[(t.half * 32 + p) * static_cast<long long>(g.N) + t.row] = p & 1 ? v.y : v.x;
+      }
   }
-  ck_cp_wait();
+  ck_cp_wait<0>();
   tcgen05_fence_before_sync();
   __syncthreads();
-  if (t.warp == 0) tmem_dealloc(tmem, TM_COLS);
+  if (t.warp == 0) tmem_dealloc(tail->tmem, TM_COLS);
 }
 
 // ---------------------------------------------------------------------------
@@ -544,6 +705,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
   const __half* raw = static_cast<const __half*>(g.raw) + h;
   const __half* Bm = static_cast<const __half*>(g.Bm) + static_cast<size_t>(grp) * g.N;
   const float bias = static_cast<const float*>(g.dt_bias)[h], rate = -expf(static_cast<const float*>(g.A_log)[h]);
+  if (threadIdx.x == 0) tail->rate = rate;
   float raw_next = 0.f;
   auto fetch = [&](long long t0) {      // whole chunks: a range that others follow is a multiple of them
     fetch_tile<2>(base + CK_B, Bm + t0 * g.bcp, g.bcp, CQ, g.N);
@@ -552,9 +714,10 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
     raw_next = __half2float(raw[(t0 + t.row) * g.rp]);
   };
   fetch(sp.lo);
-  float S[32], left = 1.f;
+  f2 S[16];
+  float left = 1.f;
 #pragma unroll
-  for (int p = 0; p < 32; ++p) S[p] = 0.f;
+  for (int p = 0; p < 16; ++p) S[p] = 0;
   const uint64_t d_bt = umma_smem_desc(base + CK_B, CK_HALF, 1024), d_t = umma_smem_desc(base + CK_T, CK_HALF, 1024);
   constexpr uint32_t id_s = umma_instr_desc(UMMA_FMT_F16, 1, 1, 128, CP), HALF_U = CK_HALF / 16, ROWS_U = 16 * 128 / 16;
   tcgen05_fence_before_sync();
@@ -564,44 +727,43 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
   uint32_t finished = 0;
   const bool odd = !(fabsf(rate) < INFINITY);
   for (long long t0 = sp.lo; t0 < sp.hi; t0 += CQ) {
-    ck_cp_wait();
+    ck_cp_wait<0>();
     fence_proxy_async_smem();
     __syncthreads();
     if (tail->abort != 0) break;
     const StepSizes z = step_sizes(raw_next, bias, rate, true, t.lane);
-    if (t.half == 0 && (t.lane & 7) == 7) tail->piece[t.row >> 3] = expf(static_cast<float>(z.end));
-    uint4 xv[4];
-    const float x_most = load_x(base + CK_X, t, xv);
-    uint32_t bm = 0;      // an infinity in B, against the two terms of V, would be a NaN
+    if (t.half == 0 && (t.lane & 7) == 7) tail->piece[t.row >> 3] = z.piece;
+    const uint32_t xm = warp_most(abs_bits(most_x(base + CK_X))), dm = warp_most(abs_bits(z.dt));
+    float m = 0.f;
     {
-      __half2 m = __float2half2_rn(0.f);
+      __half2 b2 = __float2half2_rn(0.f);      // an infinity in B, against the two terms of V, would be a NaN
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const uint4 b = ck_ld(base + CK_B + t.half * CK_HALF + ck_at(t.row, k));
         const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[e])));
+        for (int e = 0; e < 4; ++e) b2 = __hmax2_nan(b2, __habs2(*reinterpret_cast<const __half2*>(&w[e])));
       }
-      const float2 f = __half22float2(m);
-      if (!(f.x < INFINITY && f.y < INFINITY)) bm = 0x7fffffffu;
+      const float2 f = __half22float2(b2);
+      if (!(f.x < INFINITY && f.y < INFINITY)) m = INFINITY;
     }
-    const uint32_t vm = warp_most(max(bm, abs_bits(x_most * z.dt)));
-    if (t.lane == 0) tail->most[1][t.warp] = vm;
+    const uint32_t bm = warp_most(abs_bits(m));
+    if (t.lane == 0) { tail->most[1][t.warp] = max(xm, bm); tail->most[3][t.warp] = dm; }
     __syncthreads();
-    const uint32_t v_most = cta_most(tail->most[1]);
-    float after = 1.f, total = 1.f;
+    const uint32_t v_most = abs_bits(__uint_as_float(cta_most(tail->most[1])) * __uint_as_float(cta_most(tail->most[3])));
+    float w = z.dt * z.leave, total = 1.f;
 #pragma unroll
     for (int k = 0; k < CQ / 8; ++k) {
       const float d = tail->piece[k];
       total *= d;
-      if (k > (t.row >> 3)) after *= d;
+      if (k > (t.row >> 3)) w *= d;
     }
     left *= total;
     if (odd || ck_infinite(v_most)) {
-      chunk_plain<false>(ck_smem, base, t, S, z.dt, rate, CQ, nullptr, 0, pcols);
+      chunk_plain<false>(ck_smem, tail, t, S, z.dt, CQ, nullptr, 0, pcols);
     } else {
       const Scale sv = ck_scale(v_most);
-      store_v(base + CK_T, t, xv, z.dt * z.behind() * after * sv.up);
+      store_v(base + CK_T, base + CK_X, t.row, t.half, w * sv.up);
       fence_proxy_async_smem();
       tcgen05_fence_before_sync();
       __syncthreads();
@@ -613,14 +775,10 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
         umma_commit(tail->bar + 2);
       }
       __syncwarp();
-      (void)mbar_wait_abortable(tail->bar + 2, finished, a.status, &tail->abort);
+      ck_wait(tail->bar + 2, finished, a.status, &tail->abort);
       finished ^= 1;
       tcgen05_fence_after_sync();
-      float v[32];
-      tmem_ld_32x32(tq + t.half * 32, reinterpret_cast<uint32_t*>(v));
-      tmem_ld_wait();
-#pragma unroll
-      for (int p = 0; p < 32; ++p) S[p] = total * S[p] + v[p] * sv.down;
+      add_state(S, tq + t.half * 32, total, sv.down);
     }
     if (t0 + CQ < sp.hi) {
       __syncthreads();
@@ -630,10 +788,14 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
   mp_launch_dependents();
   const size_t at = static_cast<size_t>(id) * units + unit;
 #pragma unroll
-  for (int p = 0; p < 32; ++p) a.local[at * CP * CN + (t.half * 32 + p) * CN + t.row] = S[p];
+  for (int p = 0; p < 16; ++p) {
+    const float2 v = upk(S[p]);
+    a.local[at * CP * CN + (t.half * 32 + 2 * p) * CN + t.row] = v.x;
+    a.local[at * CP * CN + (t.half * 32 + 2 * p + 1) * CN + t.row] = v.y;
+  }
   // not zero, however many steps: an infinite state stays infinite then, as it does step by step
   if (threadIdx.x == 0) a.decay[at] = fmaxf(left, __int_as_float(1));
-  ck_cp_wait();
+  ck_cp_wait<0>();
   tcgen05_fence_before_sync();
   __syncthreads();
   if (t.warp == 0) tmem_dealloc(tmem, CP);
