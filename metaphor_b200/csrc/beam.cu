@@ -4,14 +4,18 @@
 // the logits, so the first kernel reads them once and leaves, per piece of a row, the maximum, the sum of exponentials below it (online) and the
 // 32 best logits; the second adds the pieces up, forms the scores in r64 and merges the beams.
 //
-// A list of 32 lies in a warp's lanes, best first.  While a row streams by, a value has to beat the list's last wanted place to be looked at
-// again (for random rows `picks` x ln(values / picks) of them do).  Two lists are merged by one bitonic stage and a bitonic sort of 32.
+// The best of a piece.  While it streams by, a thread keeps its own maximum only.  Sorted inside a warp, the maxima give a bound that at least
+// `picks` values reach: the least of the warps' values at place ceil(picks / warps).  Threads whose maximum reaches it (some tens of 256) look
+// at their values again, which the L2 still has, and put those that reach it on a list in shared memory; one warp sorts it, 32 at a time, by
+// bitonic stages.  So what is done for every value is one exponential, its sum and a comparison.  Where the list would overflow (rows of few
+// different values), every value is offered to a warp's list of 32 in turn instead.
 #include "mp_common.cuh"
 
 namespace {
 
 constexpr int BM_THREADS = 256, BM_WARPS = BM_THREADS / 32;
 constexpr int BM_LIST = 32;
+constexpr int BM_HELD = 512;             // values on a CTA's list
 constexpr int BM_NONE = 0x7fffffff;      // token of an empty place
 constexpr int BM_MAX_BEAMS = 64;
 
@@ -37,6 +41,30 @@ __device__ __forceinline__ void merge_lists(Entry<V>& a, const Entry<V>& b, int 
     const bool upper = (lane & o) != 0;  // keeps the worse one
     if (better(other, a) != upper) a = other;
   }
+}
+// A warp's entries, best first.
+template <typename V>
+__device__ __forceinline__ void sort_list(Entry<V>& a, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const Entry<V> other = entry_xor(a, o);
+      const bool worse = ((lane & o) != 0) != ((lane & size) != 0);      // this lane keeps the worse one
+      if (better(other, a) != worse) a = other;
+    }
+}
+template <typename V>
+__device__ __forceinline__ V sort_values(V a, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const V other = __shfl_xor_sync(0xffffffffu, a, o);
+      const bool less = ((lane & o) != 0) != ((lane & size) != 0);
+      a = (other > a) != less ? other : a;
+    }
+  return a;
 }
 // `e` takes its place in the list.
 template <typename V>
@@ -68,6 +96,38 @@ __device__ __forceinline__ double below_exp(double v) { return exp(v); }
 template <typename A> __device__ __forceinline__ A most_negative();
 template <> __device__ __forceinline__ float most_negative<float>() { return -3.402823466e+38f; }
 template <> __device__ __forceinline__ double most_negative<double>() { return -1.7976931348623157e+308; }
+
+// The largest of a pack's values (a NaN is passed over: it shows in the sum).
+template <typename T>
+__device__ __forceinline__ typename Acc<T>::type pack_most(const Pack<T>& p) {
+  typename Acc<T>::type m = mp_up(p.v[0]);
+#pragma unroll
+  for (int e = 1; e < Pack<T>::N; ++e) {
+    const auto v = mp_up(p.v[e]);
+    m = v > m || m != m ? v : m;
+  }
+  return m;
+}
+template <>
+__device__ __forceinline__ float pack_most<__half>(const Pack<__half>& p) {
+  const __half2* h = reinterpret_cast<const __half2*>(p.v);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return __half2float(__hmax(__low2half(m), __high2half(m)));
+}
+// sum += exp(v - top) for two values (r16 and r32: the arithmetic of both in one instruction each)
+__device__ __forceinline__ void add_exp2(float (&sum)[2], float top, float v0, float v1) {
+  float d0, d1;
+  asm("{\n.reg .b64 v, t, l;\nmov.b64 v, {%2, %3};\nmov.b64 t, {%4, %4};\nmov.b64 l, {%5, %5};\nadd.rn.f32x2 v, v, t;\nmul.rn.f32x2 v, v, l;\nmov.b64 {%0, %1}, v;\n}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(v0), "f"(v1), "f"(-top), "f"(1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d1));
+  asm("{\n.reg .b64 s, d;\nmov.b64 s, {%0, %1};\nmov.b64 d, {%2, %3};\nadd.rn.f32x2 s, s, d;\nmov.b64 {%0, %1}, s;\n}" : "+f"(sum[0]), "+f"(sum[1]) : "f"(d0), "f"(d1));
+}
+__device__ __forceinline__ void add_exp2(double (&sum)[2], double top, double v0, double v1) {
+  sum[0] += below_exp(v0 - top);
+  sum[1] += below_exp(v1 - top);
+}
 
 template <typename A>
 struct BeamScratch {     // per row and piece
@@ -105,10 +165,11 @@ __global__ void __launch_bounds__(BM_THREADS) beam_rows_kernel(const T* __restri
                                                                int pieces) {
   mp_grid_dependency();
   using A = typename Acc<T>::type;
-  constexpr int V = Pack<T>::N, U = 2;
+  constexpr int V = Pack<T>::N, U = 4;
   __shared__ A s_value[BM_WARPS][BM_LIST], s_top[BM_WARPS];
   __shared__ double s_sum[BM_WARPS];
-  __shared__ int s_token[BM_WARPS][BM_LIST];
+  __shared__ int s_token[BM_WARPS][BM_LIST], s_count, s_which[BM_HELD];
+  __shared__ A s_bound[BM_WARPS], s_held[BM_HELD];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x / pieces;
   const int piece = blockIdx.x % pieces;
@@ -121,57 +182,105 @@ __global__ void __launch_bounds__(BM_THREADS) beam_rows_kernel(const T* __restri
   const int each = (packs + pieces - 1) / pieces;
   const int first = min(piece * each, packs), end = min(first + each, packs);
 
-  Entry<A> list = {lowest(A(0)), BM_NONE}, last = list;
-  A top = most_negative<A>(), sum = A(0);
-  auto add = [&](A v) {
-    if (v > top) { sum *= below_exp(top - v); top = v; }
-    sum += below_exp(v - top);
+  A top = most_negative<A>(), sums[2] = {A(0), A(0)};
+  // this thread's packs, U at a time: what(pack, token of its first value)
+  auto stream = [&](auto what) {
+    for (int k0 = first + tid; k0 < end; k0 += BM_THREADS * U) {
+      Pack<T> in[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * BM_THREADS;
+        if (k < end) {
+          if (whole) {
+            in[u] = ld_pack(src, k);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) in[u].v[e] = src[static_cast<size_t>(k) * V + e];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * BM_THREADS;
+        if (k < end) what(in[u], k * V);
+      }
+    }
   };
-  for (int k0 = first; k0 < end; k0 += BM_THREADS * U) {
-    Pack<T> in[U];
-    bool have[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * BM_THREADS + tid;
-      have[u] = k < end;
-      if (have[u]) {
-        if (whole) {
-          in[u] = ld_pack_stream(src, k);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) in[u].v[e] = src[static_cast<size_t>(k) * V + e];
-        }
-      }
+  auto raise = [&](A most) {
+    if (most > top) {
+      const A f = below_exp(top - most);
+      sums[0] *= f;
+      sums[1] *= f;
+      top = most;
     }
+  };
+  stream([&](const Pack<T>& in, int) {
+    raise(pack_most(in));
+    A v[V];
+    unpack(in, v);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      A v[V], most = lowest(A(0));
-      if (have[u]) {
-        unpack(in[u], v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) most = v[e] > most ? v[e] : most;
-        if (most > top) { sum *= below_exp(top - most); top = most; }
-#pragma unroll
-        for (int e = 0; e < V; ++e) sum += below_exp(v[e] - top);
-      }
-      const int i = (k0 + u * BM_THREADS + tid) * V;
-      if (__any_sync(0xffffffffu, have[u] && (most >= last.v))) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const Entry<A> mine = have[u] ? Entry<A>{v[e], i + e} : Entry<A>{lowest(A(0)), BM_NONE};
-          offer(list, last, mine, picks, lane);
-        }
-      }
-    }
+    for (int e = 0; e < V; e += 2) add_exp2(sums, top, v[e], v[e + 1]);
+  });
+  const int at_tail = packs * V + tid;      // fewer than a pack
+  const bool has_tail = piece == 0 && tid < tail;
+  if (has_tail) {
+    const A v = mp_up(src[at_tail]);
+    raise(v);
+    sums[0] += below_exp(v - top);
   }
-  if (piece == 0 && warp == 0) {
-    const int i = packs * V + lane;
-    Entry<A> e = {lowest(A(0)), BM_NONE};
-    if (lane < tail) {
-      e = {mp_up(src[i]), i};
-      add(e.v);
+  const A sum = sums[0] + sums[1];
+  if (tid == 0) s_count = 0;
+  {
+    const A sorted = sort_values(top, lane);
+    const A at = __shfl_sync(0xffffffffu, sorted, (picks + BM_WARPS - 1) / BM_WARPS - 1);
+    if (lane == 0) s_bound[warp] = at;
+  }
+  __syncthreads();
+  A bound = s_bound[0];
+#pragma unroll
+  for (int w = 1; w < BM_WARPS; ++w) bound = s_bound[w] < bound ? s_bound[w] : bound;
+  if (bound == most_negative<A>()) bound = lowest(A(0));      // threads without a value above minus infinity have it too
+  auto take = [&](A v, int i) {
+    if (v >= bound) {
+      const int at = atomicAdd(&s_count, 1);
+      if (at < BM_HELD) { s_held[at] = v; s_which[at] = i; }
     }
-    offer(list, last, e, picks, lane);
+  };
+  if (!(top < bound)) {
+    stream([&](const Pack<T>& in, int i) {
+      if (pack_most(in) < bound) return;
+      A v[V];
+      unpack(in, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) take(v[e], i + e);
+    });
+    if (has_tail) take(mp_up(src[at_tail]), at_tail);
+  }
+  __syncthreads();
+  const int count = s_count;
+  Entry<A> list = {lowest(A(0)), BM_NONE};
+  if (count <= BM_HELD) {
+    // warp w has places 32 w ..; mostly there is work for the first ones only
+    for (int k = warp * 32; k < count; k += BM_THREADS) {
+      Entry<A> e = {lowest(A(0)), BM_NONE};
+      if (k + lane < count) e = {s_held[k + lane], s_which[k + lane]};
+      sort_list(e, lane);
+      merge_lists(list, e, lane);
+    }
+  } else {
+    Entry<A> last = list;
+    for (int k0 = first + warp * 32; k0 < end; k0 += BM_THREADS) {
+      const int k = k0 + lane;
+#pragma unroll 1
+      for (int e = 0; e < V; ++e) {
+        Entry<A> mine = {lowest(A(0)), BM_NONE};
+        if (k < end) mine = {mp_up(src[static_cast<size_t>(k) * V + e]), k * V + e};
+        offer(list, last, mine, picks, lane);
+      }
+    }
+    Entry<A> mine = {lowest(A(0)), BM_NONE};
+    if (has_tail) mine = {mp_up(src[at_tail]), at_tail};
+    offer(list, last, mine, picks, lane);
   }
   // the warp's sum, then the CTA's
   const A wtop = warp_reduce<MaxOp>(top);
@@ -180,7 +289,9 @@ __global__ void __launch_bounds__(BM_THREADS) beam_rows_kernel(const T* __restri
   s_token[warp][lane] = list.i;
   if (lane == 0) { s_top[warp] = wtop; s_sum[warp] = wsum; }
   __syncthreads();
+  const int busy = count <= BM_HELD ? (count + 31) / 32 : BM_WARPS;      // warps that have something on their lists
   for (int half = BM_WARPS / 2; half > 0; half >>= 1) {
+    if (half >= busy) continue;
     if (warp < half) {
       merge_lists(list, Entry<A>{s_value[warp + half][lane], s_token[warp + half][lane]}, lane);
       s_value[warp][lane] = list.v;
@@ -198,38 +309,71 @@ __global__ void __launch_bounds__(BM_THREADS) beam_rows_kernel(const T* __restri
   }
 }
 
-// One CTA per search.
+// One CTA per search.  `share` warps have a beam's pieces, so that few beams keep all warps busy; a warp's share of the pieces is `seats` lists
+// at a time, the first 32 / seats places of each (at least `picks`), sorted together.
+constexpr int BM_MERGE_WARPS = 16;
 template <typename A>
-__global__ void __launch_bounds__(BM_THREADS) beam_merge_kernel(BeamScratch<A> in, const A* scores, const int* finished, int eos, A* next_scores,
-                                                                int* parents, int* tokens, int* next_finished, int beams, int vocab, int picks, int pieces) {
-  mp_grid_dependency();
-  __shared__ A s_value[BM_WARPS][BM_LIST];
-  __shared__ int s_from[BM_WARPS][BM_LIST], s_key[BM_WARPS][BM_LIST];
-  __shared__ double s_score[BM_WARPS][BM_LIST];
+__global__ void __launch_bounds__(BM_MERGE_WARPS * 32) beam_merge_kernel(BeamScratch<A> in, const A* scores, const int* finished, int eos, A* next_scores,
+                                                                         int* parents, int* tokens, int* next_finished, int beams, int vocab, int picks,
+                                                                         int pieces, int share, int seats) {
+  __shared__ A s_value[BM_MERGE_WARPS][BM_LIST];
+  __shared__ int s_from[BM_MERGE_WARPS][BM_LIST], s_key[BM_MERGE_WARPS][BM_LIST];
+  __shared__ double s_score[BM_MERGE_WARPS][BM_LIST];
   __shared__ int s_token[BM_MAX_BEAMS][BM_LIST], s_done[BM_MAX_BEAMS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t search = blockIdx.x;
-  // `share` warps have a beam's pieces, so that few beams keep all warps busy
-  int share = BM_WARPS;
-  while (share > 1 && share * beams > BM_WARPS) share >>= 1;
+  const int places = BM_LIST / seats, seat = lane / places, place = lane % places;
+  const int beams_at_once = BM_MERGE_WARPS / share;
   Entry<double> best = {lowest(0.0), BM_NONE};
-  for (int b0 = 0; b0 < beams; b0 += BM_WARPS / share) {
+  mp_grid_dependency();
+  for (int b0 = 0; b0 < beams; b0 += beams_at_once) {
     const int beam = b0 + warp / share, part = warp % share;
     const bool live = beam < beams;
     const size_t row = search * beams + (live ? beam : 0);
     const A had = scores[row];
-    const bool dead = beam_dead(had), done = finished != nullptr && finished[row] != 0;
+    const bool done = finished != nullptr && finished[row] != 0, dead = beam_dead(had);
     Entry<A> list = {lowest(A(0)), BM_NONE};
+    A top = most_negative<A>();
+    double sum = 0;
     if (live && !dead && !done) {
-      for (int k = part; k < pieces; k += share) {
-        const size_t at = (row * pieces + k) * BM_LIST + lane;
-        merge_lists(list, Entry<A>{in.value[at], in.token[at]}, lane);
+      for (int k0 = part * seats; k0 < pieces; k0 += share * seats) {
+        const int k = k0 + seat;
+        Entry<A> e = {lowest(A(0)), BM_NONE};
+        if (k < pieces) {
+          const size_t at = (row * pieces + k) * BM_LIST + place;
+          e = {in.value[at], in.token[at]};
+        }
+        if (seats > 1) sort_list(e, lane);
+        if (k0 == part * seats) list = e;
+        else merge_lists(list, e, lane);
+      }
+      if (part == 0) {      // the pieces' sums under one maximum
+        for (int k = lane; k < pieces; k += 32) {
+          const A t = in.top[row * pieces + k];
+          const double more = in.sum[row * pieces + k];
+          const A both = t > top ? t : top;
+          sum = sum * static_cast<double>(below_exp(top - both)) + more * static_cast<double>(below_exp(t - both));
+          top = both;
+        }
+        const A all = warp_reduce<MaxOp>(top);
+        sum = warp_reduce<SumOp>(sum * static_cast<double>(below_exp(top - all)));
+        top = all;
       }
     }
-    __syncthreads();      // the lists of the beams before have been read
-    s_value[warp][lane] = list.v;
-    s_from[warp][lane] = list.i;
-    __syncthreads();
+    if (share > 1) {
+      if (b0 != 0) __syncthreads();      // the lists of the beams before have been read
+      s_value[warp][lane] = list.v;
+      s_from[warp][lane] = list.i;
+      __syncthreads();
+      for (int half = share / 2; half > 0; half >>= 1) {
+        if (part < half) {
+          merge_lists(list, Entry<A>{s_value[warp + half][lane], s_from[warp + half][lane]}, lane);
+          s_value[warp][lane] = list.v;
+          s_from[warp][lane] = list.i;
+        }
+        if (half > 1) __syncthreads();
+      }
+    }
     if (live && part == 0) {
       double score = lowest(0.0);
       if (dead) {
@@ -237,28 +381,26 @@ __global__ void __launch_bounds__(BM_THREADS) beam_merge_kernel(BeamScratch<A> i
       } else if (done) {
         list.i = lane == 0 ? eos : lane - 1 < eos ? lane - 1 : lane;
         if (lane == 0) score = static_cast<double>(had);
-      } else {
-        for (int k = 1; k < share; ++k) merge_lists(list, Entry<A>{s_value[warp + k][lane], s_from[warp + k][lane]}, lane);
-        A top = most_negative<A>();
-        for (int k = lane; k < pieces; k += 32) { const A t = in.top[row * pieces + k]; top = t > top ? t : top; }
-        top = warp_reduce<MaxOp>(top);
-        double sum = 0;
-        for (int k = lane; k < pieces; k += 32) sum += in.sum[row * pieces + k] * static_cast<double>(below_exp(in.top[row * pieces + k] - top));
-        sum = warp_reduce<SumOp>(sum);
-        // a NaN or an infinity among the logits, or nothing above minus infinity: no probabilities
-        if (sum > 0 && sum < 1.0 / 0.0) score = static_cast<double>(had) + (static_cast<double>(list.v) - (static_cast<double>(top) + log(sum)));
-        else list.i = lane;
+      } else if (sum > 0 && sum < 1.0 / 0.0) {
+        score = static_cast<double>(had) + (static_cast<double>(list.v) - (static_cast<double>(top) + log(sum)));
+        if (score != score) score = lowest(0.0);      // an infinite score behind a token that is ruled out
+      } else {      // a NaN or an infinity among the logits, or nothing above minus infinity: no probabilities
+        list.i = lane;
       }
       s_token[beam][lane] = list.i;
       if (lane == 0) s_done[beam] = done;
       const bool wanted = lane < picks;
-      merge_lists(best, Entry<double>{wanted ? score : lowest(0.0), wanted ? beam * BM_LIST + lane : BM_NONE}, lane);
+      const Entry<double> e = {wanted ? score : lowest(0.0), wanted ? beam * BM_LIST + lane : BM_NONE};
+      if (b0 == 0) best = e;
+      else merge_lists(best, e, lane);
     }
   }
+  // the warps with beams: every `share`-th
   s_score[warp][lane] = best.v;
   s_key[warp][lane] = best.i;
   __syncthreads();
-  for (int half = BM_WARPS / 2; half > 0; half >>= 1) {
+  for (int half = BM_MERGE_WARPS / 2; half >= share; half >>= 1) {
+    if (half >= beams * share) continue;
     if (warp < half) {
       merge_lists(best, Entry<double>{s_score[warp + half][lane], s_key[warp + half][lane]}, lane);
       s_score[warp][lane] = best.v;
@@ -295,10 +437,13 @@ void beam_select_impl(const void* logits, len_t logits_pitch, const void* scores
       beam_rows_kernel<T>, static_cast<const T*>(logits), logits_pitch, static_cast<const A*>(scores), static_cast<const int*>(finished), sc,
       static_cast<int>(vocab), static_cast<int>(picks), pieces);
   MP_LAUNCH_CHECK();
-  MpLaunch(static_cast<unsigned>(batch), BM_THREADS, 0, mp_stream(ctx))(
+  int share = 1, seats = 1;
+  while (share < BM_MERGE_WARPS && 2 * share * static_cast<int>(beams) <= BM_MERGE_WARPS && share < pieces) share <<= 1;
+  while (2 * seats * static_cast<int>(picks) <= BM_LIST && seats < pieces) seats <<= 1;
+  MpLaunch(static_cast<unsigned>(batch), BM_MERGE_WARPS * 32, 0, mp_stream(ctx))(
       beam_merge_kernel<A>, sc, static_cast<const A*>(scores), static_cast<const int*>(finished), eos < vocab ? static_cast<int>(eos) : -1,
       static_cast<A*>(next_scores), static_cast<int*>(parents), static_cast<int*>(tokens), static_cast<int*>(next_finished), static_cast<int>(beams),
-      static_cast<int>(vocab), static_cast<int>(picks), pieces);
+      static_cast<int>(vocab), static_cast<int>(picks), pieces, share, seats);
   MP_LAUNCH_CHECK();
 }
 
