@@ -23,12 +23,97 @@ __device__ __forceinline__ void st_vec(T* p, const typename Acc<T>::type* in) {
 }
 
 // pre * sigmoid(pre).  r16 results have 11 bits: the special-function unit's exponential and reciprocal (22 bits) lose nothing there.
-template <typename T> __device__ __forceinline__ typename Acc<T>::type silu_of(typename Acc<T>::type v) { return v / (typename Acc<T>::type(1) + seq_exp(-v)); }
-template <> __device__ __forceinline__ float silu_of<__half>(float v) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return v * r;
+template <typename T, int V>
+__device__ __forceinline__ StVec<T, V> silu_vec(const typename Acc<T>::type (&v)[V]) {
+  StVec<T, V> x;
+  if constexpr (std::is_same<T, __half>::value) {
+    float r[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float t;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(v[e] * -1.4426950408889634f));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(1.f + t));
+      r[e] = v[e] * t;
+    }
+    if constexpr (V % 2 == 0) {
+      __half2* h = reinterpret_cast<__half2*>(x.v);
+#pragma unroll
+      for (int e = 0; e < V; e += 2) h[e / 2] = __floats2half2_rn(r[e], r[e + 1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x.v[e] = __float2half_rn(r[e]);
+    }
+  } else {
+    using A = typename Acc<T>::type;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x.v[e] = mp_down<T>(v[e] / (A(1) + seq_exp(-v[e])));
+  }
+  return x;
+}
+
+// The taps of V neighbouring channels lie in a row: as many whole vectors as there are taps.
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_taps(const T* __restrict__ w, int c, typename Acc<T>::type (&tap)[W][V]) {
+  typename Acc<T>::type flat[W * V];
+#pragma unroll
+  for (int k = 0; k < W; ++k) ld_vec<T, V>(w + static_cast<size_t>(c) * W + k * V, flat + k * V);
+#pragma unroll
+  for (int k = 0; k < W; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) tap[k][e] = flat[e * W + k];
+}
+
+// acc += a b, value by value; fp32 values two at a time.
+template <int V>
+__device__ __forceinline__ void fma_vec(float (&acc)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2)
+      asm("{\n.reg .b64 c, a, b;\nmov.b64 c, {%0, %1};\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nfma.rn.f32x2 c, a, b, c;\nmov.b64 {%0, %1}, c;\n}"
+          : "+f"(acc[e]), "+f"(acc[e + 1])
+          : "f"(a[e]), "f"(a[e + 1]), "f"(b[e]), "f"(b[e + 1]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] += a[e] * b[e];
+  }
+}
+template <int V>
+__device__ __forceinline__ void fma_vec(double (&acc)[V], const double (&a)[V], const double (&b)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] += a[e] * b[e];
+}
+template <int V>
+__device__ __forceinline__ void mul_vec(float (&out)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2)
+      asm("{\n.reg .b64 c, a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 c, a, b;\nmov.b64 {%0, %1}, c;\n}"
+          : "=f"(out[e]), "=f"(out[e + 1])
+          : "f"(a[e]), "f"(a[e + 1]), "f"(b[e]), "f"(b[e + 1]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = a[e] * b[e];
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_vec(double (&out)[V], const double (&a)[V], const double (&b)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) out[e] = a[e] * b[e];
+}
+template <typename T, int V>
+__device__ __forceinline__ void widen(const StVec<T, V>& x, typename Acc<T>::type (&out)[V]) {
+  if constexpr (std::is_same<T, __half>::value && V % 2 == 0) {
+    const __half2* h = reinterpret_cast<const __half2*>(x.v);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 f = __half22float2(h[e / 2]);
+      out[e] = f.x;
+      out[e + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = mp_up(x.v[e]);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -36,10 +121,10 @@ template <> __device__ __forceinline__ float silu_of<__half>(float v) {
 // Rows that reach into the kept state (the first W - 1 of a sequence) belong to the thread that has the sequence's first row, even behind its
 // run's end, and that thread writes the new state too, from inputs that it fetches again: so nobody else reads what it overwrites.
 // ---------------------------------------------------------------------------
-constexpr int CS_TX = 32, CS_TY = 4;
+constexpr int CS_TX = 32, CS_TY = 4, CS_U = 8;
 
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(CS_TX * CS_TY) conv_prompt_kernel(const T* __restrict__ x, size_t xp, const T* __restrict__ w, const T* __restrict__ bias,
+__global__ void __launch_bounds__(CS_TX * CS_TY, 4) conv_prompt_kernel(const T* __restrict__ x, size_t xp, const T* __restrict__ w, const T* __restrict__ bias,
                                                                     T* __restrict__ states, T* __restrict__ y, size_t yp, const Sequences q, int channels,
                                                                     int run) {
   mp_grid_dependency();
@@ -50,12 +135,11 @@ __global__ void __launch_bounds__(CS_TX * CS_TY) conv_prompt_kernel(const T* __r
   const long long r0 = static_cast<long long>(piece) * run, r1 = min(r0 + run, q.rows);
   A tap[W][V], b[V];
   if (live) {
+    if (bias != nullptr) ld_vec<T, V>(bias + c, b);
+    else
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      b[e] = bias != nullptr ? mp_up(bias[c + e]) : A(0);
-#pragma unroll
-      for (int k = 0; k < W; ++k) tap[k][e] = mp_up(w[static_cast<size_t>(c + e) * W + k]);
-    }
+      for (int e = 0; e < V; ++e) b[e] = A(0);
+    load_taps<T, V, W>(w, c, tap);
   }
   // a sequence without rows keeps nothing but zeros where it does not go on; they are dealt out over the pieces
   for (int s = piece; s < q.nseq; s += pieces) {
@@ -73,39 +157,30 @@ __global__ void __launch_bounds__(CS_TX * CS_TY) conv_prompt_kernel(const T* __r
   for (; s < q.nseq && at < r1; ++s) {
     const long long lo = seq_first(q, s), hi = seq_first(q, s + 1), slot = seq_slot(q.slots, q.nslots, s);
     if (hi <= at || slot < 0) { at = max(at, hi); continue; }
-    A h[W - 1][V];
+    StVec<T, V> before[W - 1] = {};
     long long end;
     if (lo >= at) {      // its first row is here
       at = lo;
       if (at >= r1) break;
       T* kept = states + slot * (W - 1) * channels + c;
       if (live) {
+        if (seq_resumes(q, s))
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) {
-          if (seq_resumes(q, s)) ld_vec<T, V>(kept + static_cast<size_t>(k) * channels, h[k]);
-          else
-#pragma unroll
-            for (int e = 0; e < V; ++e) h[k][e] = A(0);
-        }
-        A last[W - 1][V];
+          for (int k = 0; k < W - 1; ++k) before[k] = *reinterpret_cast<const StVec<T, V>*>(kept + static_cast<size_t>(k) * channels);
+        StVec<T, V> last[W - 1] = {};
         const long long len = hi - lo;
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) {
           const long long p = len - (W - 1) + k;      // in the sequence; before it lies what was kept
           if (p >= 0) {
-            ld_vec<T, V>(x + (lo + p) * xp + c, last[k]);
+            last[k] = *reinterpret_cast<const StVec<T, V>*>(x + (lo + p) * xp + c);
           } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) last[k][e] = A(0);
-#pragma unroll
-            for (int j = 1; j < W - 1; ++j)           // p + W - 1 = len + k < W - 1
-              if (j == len + k)
-#pragma unroll
-                for (int e = 0; e < V; ++e) last[k][e] = h[j][e];
+            if (k + 1 < W - 1 && len == 1) last[k] = before[k + 1 < W - 1 ? k + 1 : 0];
+            if (k + 2 < W - 1 && len == 2) last[k] = before[k + 2 < W - 1 ? k + 2 : 0];
           }
         }
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) st_vec<T, V>(kept + static_cast<size_t>(k) * channels, last[k]);
+        for (int k = 0; k < W - 1; ++k) *reinterpret_cast<StVec<T, V>*>(kept + static_cast<size_t>(k) * channels) = last[k];
       }
       end = min(hi, max(r1, lo + W - 1));
     } else {
@@ -113,39 +188,42 @@ __global__ void __launch_bounds__(CS_TX * CS_TY) conv_prompt_kernel(const T* __r
       end = min(hi, r1);
       if (at < end && live) {
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) ld_vec<T, V>(x + (at - (W - 1) + k) * xp + c, h[k]);
+        for (int k = 0; k < W - 1; ++k) before[k] = *reinterpret_cast<const StVec<T, V>*>(x + (at - (W - 1) + k) * xp + c);
       }
     }
     if (live) {
-      constexpr int U = 4;
-      for (; at < end; at += U) {
-        A in[U][V];
+      constexpr int U = CS_U;
+      A h[W - 1][V];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (at + u < end) ld_vec<T, V>(x + (at + u) * xp + c, in[u]);
+      for (int k = 0; k < W - 1; ++k) widen(before[k], h[k]);
+      const T* from = x + at * xp + c;
+      T* to = y + at * yp + c;
+      for (int left = static_cast<int>(end - at); left > 0; left -= U) {
+        StVec<T, V> in[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (at + u < end) {
-            A out[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              A pre = b[e];
-#pragma unroll
-              for (int k = 0; k < W - 1; ++k) {
-                const int j = u - (W - 1) + k;      // input of tap k: in this group, or before it
-                pre += tap[k][e] * (j >= 0 ? in[j >= 0 ? j : 0][e] : h[j < 0 ? j + W - 1 : 0][e]);
-              }
-              pre += tap[W - 1][e] * in[u][e];
-              out[e] = silu_of<T>(pre);
-            }
-            st_vec<T, V>(y + (at + u) * yp + c, out);
-          }
+          if (u < left) in[u] = *reinterpret_cast<const StVec<T, V>*>(from);
+          from += xp;
         }
-        if (at + U < end) {
+        // (rows behind the last are worked out too, from whatever is there: without a branch around each the taps' inputs move on by name)
 #pragma unroll
-          for (int k = 0; k < W - 1; ++k)
+        for (int u = 0; u < U; ++u) {
+          A now[V], pre[V];
+          widen(in[u], now);
 #pragma unroll
-            for (int e = 0; e < V; ++e) h[k][e] = in[U - (W - 1) + k][e];
+          for (int e = 0; e < V; ++e) pre[e] = b[e];
+#pragma unroll
+          for (int k = 0; k < W - 1; ++k) fma_vec(pre, tap[k], h[k]);
+          fma_vec(pre, tap[W - 1], now);
+          const StVec<T, V> out = silu_vec<T, V>(pre);
+          if (u < left) *reinterpret_cast<StVec<T, V>*>(to) = out;
+          to += yp;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+#pragma unroll
+            for (int k = 0; k + 1 < W - 1; ++k) h[k][e] = h[k + 1][e];
+            h[W - 2][e] = now[e];
+          }
         }
       }
     }
@@ -168,88 +246,127 @@ __global__ void __launch_bounds__(128) conv_token_kernel(const T* x, size_t xp, 
   const long long slot = seq_slot(slots, nslots, r);
   if (slot < 0) return;
   T* kept = states + slot * (W - 1) * channels + c;
-  A in[W][V], out[V];
+  A in[W][V], tap[W][V], b[V] = {};
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) ld_vec<T, V>(kept + static_cast<size_t>(k) * channels, in[k]);
   ld_vec<T, V>(x + r * xp + c, in[W - 1]);
+  load_taps<T, V, W>(w, c, tap);
+  if (bias != nullptr) ld_vec<T, V>(bias + c, b);
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    A pre = bias != nullptr ? mp_up(bias[c + e]) : A(0);
-#pragma unroll
-    for (int k = 0; k < W; ++k) pre += mp_up(w[static_cast<size_t>(c + e) * W + k]) * in[k][e];
-    out[e] = silu_of<T>(pre);
-  }
+  for (int k = 0; k < W; ++k) fma_vec(b, tap[k], in[k]);
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) st_vec<T, V>(kept + static_cast<size_t>(k) * channels, in[k + 1]);
-  st_vec<T, V>(y + r * yp + c, out);
+  *reinterpret_cast<StVec<T, V>*>(y + r * yp + c) = silu_vec<T, V>(b);
 }
 
 // ---------------------------------------------------------------------------
 // Scan of one token per sequence:  S = exp(dt A) S + dt x (x) B,  y = S C.  The state ([P][N], accumulator type) is read and written once and
-// is nearly all of the traffic.  `width` lanes have a row p of it, V values at a time; a warp has U rows per lane group in flight.
+// is nearly all of the traffic.  L lanes have a row p of it, V values at a time; a warp takes ST_U rows per lane group at a time, `batches` times,
+// so that what a row costs beside its own values (step size, B and C, addresses) is shared.  The ST_U sums of a lane group are added up across
+// its lanes by halves: in each of three rounds a lane hands on half of its sums and keeps the others.
 // ---------------------------------------------------------------------------
 constexpr int ST_U = 8;
 
-template <typename T, int V>
-__global__ void __launch_bounds__(128) scan_token_kernel(const T* __restrict__ x, size_t xp, const T* __restrict__ raw, size_t rp,
+// The sum over the L lanes of a group of s[u]; returns that of row u = the lane's number in the group / (L / 8), for L < 8 that of row
+// u = lane * (8 / L) + k in s[k].
+template <int L, typename A>
+__device__ __forceinline__ void sum_rows(A (&s)[ST_U], int lane) {
+  int have = ST_U;
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) {
+    if (have > 1) {
+      have >>= 1;
+      const bool up = (lane & o) != 0;
+#pragma unroll
+      for (int k = 0; k < ST_U / 2; ++k)
+        if (k < have) {
+          const A send = up ? s[k] : s[k + have], keep = up ? s[k + have] : s[k];
+          s[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    } else {
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+    }
+  }
+}
+
+template <typename T, int V, int L>
+__global__ void __launch_bounds__(128, sizeof(T) == 8 ? 3 : 6) scan_token_kernel(const T* __restrict__ x, size_t xp, const T* __restrict__ raw, size_t rp,
                                                          const typename Acc<T>::type* __restrict__ dt_bias, const typename Acc<T>::type* __restrict__ A_log,
                                                          const T* __restrict__ Bm, const T* __restrict__ Cm, size_t bcp,
                                                          typename Acc<T>::type* __restrict__ states, const int* __restrict__ slots, T* __restrict__ y,
-                                                         size_t yp, long long nslots, int H, int P, int N, int G, int width, int splits) {
+                                                         size_t yp, long long nslots, int H, int P, int N, int G, int batches, int splits) {
   mp_grid_dependency();
   using A = typename Acc<T>::type;
+  constexpr int GROUPS = 32 / L, ROWS = ST_U * GROUPS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int split = blockIdx.x % splits;
-  const long long rh = blockIdx.x / splits, r = rh / H;
-  const int h = static_cast<int>(rh % H);
-  const long long slot = seq_slot(slots, nslots, r);
-  if (slot < 0) return;
-  const int groups = 32 / width, sub = lane / width, n0 = (lane % width) * V;
-  const int p0 = (split * warps + warp) * ST_U * groups + sub;      // rows p0, p0 + groups, ...
-  if (p0 - sub >= P) return;
-  A* state = states + (slot * H + h) * static_cast<long long>(P) * N;
-  const A dt = seq_softplus(mp_up(raw[r * rp + h]) + dt_bias[h]);
-  const A decay = seq_exp(dt * -seq_exp(A_log[h]));
+  const unsigned split = blockIdx.x % splits, rh = blockIdx.x / splits, r = rh / H, h = rh % H;
+  const int sub = lane / L, n0 = (lane % L) * V;
+  const int first = (split * warps + warp) * batches * ROWS;      // rows first + u GROUPS + sub
+  if (first >= P) return;
+  const A step = mp_up(raw[r * rp + h]) + dt_bias[h], rate = A_log[h];
   const T* b = Bm + r * bcp + static_cast<size_t>(h / (H / G)) * N;
   const T* cc = Cm + r * bcp + static_cast<size_t>(h / (H / G)) * N;
-  A xd[ST_U], sum[ST_U];
+  const T* xr = x + r * xp + static_cast<size_t>(h) * P;
+  T* yr = y + r * yp + static_cast<size_t>(h) * P;
+  StVec<T, V> braw, craw;
+  auto fetch_bc = [&](int n) {
 #pragma unroll
-  for (int u = 0; u < ST_U; ++u) {
-    const int p = p0 + u * groups;
-    xd[u] = p < P ? dt * mp_up(x[r * xp + static_cast<size_t>(h) * P + p]) : A(0);
-    sum[u] = A(0);
-  }
-  for (int n = n0; n - n0 < N; n += width * V) {
-    StVec<A, V> s[ST_U];
-#pragma unroll
-    for (int u = 0; u < ST_U; ++u) {
-      const int p = p0 + u * groups;
-      if (p < P && n < N) s[u] = *reinterpret_cast<const StVec<A, V>*>(state + static_cast<size_t>(p) * N + n);
-    }
-    A bv[V], cv[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      bv[e] = n < N ? mp_up(b[n + e]) : A(0);
-      cv[e] = n < N ? mp_up(cc[n + e]) : A(0);
-    }
+    for (int e = 0; e < V; ++e) { braw.v[e] = n < N ? b[n + e] : T(0.f); craw.v[e] = n < N ? cc[n + e] : T(0.f); }
+  };
+  fetch_bc(n0);
+  const long long slot = seq_slot(slots, nslots, r);
+  if (slot < 0) return;
+  A* state = states + (slot * H + h) * static_cast<long long>(P) * N;
+  A dt, decay[V];
+  bool begun = false;
+  for (int p0 = first; p0 < min(P, first + batches * ROWS); p0 += ROWS) {
+    A sum[ST_U], xd[ST_U];
 #pragma unroll
     for (int u = 0; u < ST_U; ++u) {
-      const int p = p0 + u * groups;
-      if (p < P && n < N) {
+      sum[u] = A(0);
+      const int p = p0 + u * GROUPS + sub;
+      xd[u] = p < P ? mp_up(xr[p]) : A(0);
+    }
+    for (int n = n0; n - n0 < N; n += L * V) {
+      StVec<A, V> s[ST_U];
+      A* at = state + static_cast<size_t>(p0 + sub) * N + n;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          s[u].v[e] = decay * s[u].v[e] + xd[u] * bv[e];
-          sum[u] += s[u].v[e] * cv[e];
+      for (int u = 0; u < ST_U; ++u)
+        if (p0 + u * GROUPS + sub < P && n < N) s[u] = *reinterpret_cast<const StVec<A, V>*>(at + static_cast<size_t>(u * GROUPS) * N);
+      if (!begun) {      // while the first values are on their way
+        dt = seq_softplus(step);
+        const A d = seq_exp(dt * -seq_exp(rate));
+#pragma unroll
+        for (int e = 0; e < V; ++e) decay[e] = d;
+        begun = true;
+      }
+      if (N > L * V) fetch_bc(n);
+      A bv[V], cv[V];
+      widen(braw, bv);
+      widen(craw, cv);
+#pragma unroll
+      for (int u = 0; u < ST_U; ++u) {
+        if (p0 + u * GROUPS + sub < P && n < N) {
+          A xv[V], now[V], part[V];
+          const A d = dt * xd[u];
+#pragma unroll
+          for (int e = 0; e < V; ++e) xv[e] = d;
+          mul_vec(now, decay, s[u].v);
+          fma_vec(now, xv, bv);
+          mul_vec(part, now, cv);
+#pragma unroll
+          for (int e = 0; e < V; ++e) { s[u].v[e] = now[e]; sum[u] += part[e]; }
+          *reinterpret_cast<StVec<A, V>*>(at + static_cast<size_t>(u * GROUPS) * N) = s[u];
         }
-        *reinterpret_cast<StVec<A, V>*>(state + static_cast<size_t>(p) * N + n) = s[u];
       }
     }
-  }
+    sum_rows<L>(sum, lane);
+    constexpr int HELD = L >= ST_U ? 1 : ST_U / L, SHARED = L >= ST_U ? L / ST_U : 1;      // sums of a lane, lanes with the same one
 #pragma unroll
-  for (int u = 0; u < ST_U; ++u) {
-    for (int o = width >> 1; o > 0; o >>= 1) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
-    const int p = p0 + u * groups;
-    if (p < P && lane % width == 0) y[r * yp + static_cast<size_t>(h) * P + p] = mp_down<T>(sum[u]);
+    for (int k = 0; k < HELD; ++k) {
+      const int u = (lane % L) / SHARED * HELD + k, p = p0 + u * GROUPS + sub;
+      if (lane % SHARED == 0 && p < P) yr[p] = mp_down<T>(sum[k]);
+    }
   }
 }
 
@@ -297,10 +414,9 @@ bool fits(len_t v) { return v <= 0x7fffffffull; }
 template <typename T, int V>
 void conv_prompt_run(const T* x, size_t xp, const T* w, const T* bias, T* states, T* y, size_t yp, const Sequences& q, int channels, int width, StreamContext ctx) {
   const int cols = (channels + V * CS_TX - 1) / (V * CS_TX);
-  // runs of 16 rows read 19; shorter ones where there are too few threads for every SM
-  int run = 16;
-  const long long enough = static_cast<long long>(mp_sm_count(ctx)) * 8;
-  while (run > 4 && static_cast<long long>(cols) * ((q.rows + run * CS_TY - 1) / (run * CS_TY)) < enough) run >>= 1;
+  // Rows of a run so that four CTAs on each SM, as many as fit, take all of them at once; a run reads W - 1 rows more than it writes.
+  const long long per_sm = (q.rows * cols + 16ll * mp_sm_count(ctx) - 1) / (16ll * mp_sm_count(ctx));
+  int run = static_cast<int>(per_sm < 4 ? 4 : per_sm > 32 ? 32 : per_sm);
   long long tiles = (q.rows + static_cast<long long>(run) * CS_TY - 1) / (static_cast<long long>(run) * CS_TY);
   while (tiles > 65535) { run *= 2; tiles = (q.rows + static_cast<long long>(run) * CS_TY - 1) / (static_cast<long long>(run) * CS_TY); }
   const dim3 grid(cols, static_cast<unsigned>(tiles < 1 ? 1 : tiles)), block(CS_TX, CS_TY);
@@ -332,7 +448,7 @@ void causal_conv1d_silu_prompt_impl(const void* x, len_t x_pitch, const void* w,
   constexpr int PN = Pack<T>::N;
   const T *xt = static_cast<const T*>(x), *wt = static_cast<const T*>(w), *bt = static_cast<const T*>(bias);
   T *st = static_cast<T*>(states), *yt = static_cast<T*>(y);
-  if (mp_aligned16(x) && mp_aligned16(y) && mp_aligned16(states) && x_pitch % PN == 0 && y_pitch % PN == 0 && channels % PN == 0)
+  if (mp_aligned16(x) && mp_aligned16(w) && (bias == nullptr || mp_aligned16(bias)) && mp_aligned16(y) && mp_aligned16(states) && x_pitch % PN == 0 && y_pitch % PN == 0 && channels % PN == 0)
     conv_prompt_run<T, PN>(xt, x_pitch, wt, bt, st, yt, y_pitch, q, static_cast<int>(channels), static_cast<int>(width), ctx);
   else
     conv_prompt_run<T, 1>(xt, x_pitch, wt, bt, st, yt, y_pitch, q, static_cast<int>(channels), static_cast<int>(width), ctx);
@@ -361,7 +477,7 @@ void causal_conv1d_silu_token_impl(const void* x, len_t x_pitch, const void* w, 
   T *st = static_cast<T*>(states), *yt = static_cast<T*>(y);
   const int* sl = static_cast<const int*>(slots);
   const long long r = static_cast<long long>(rows), n = static_cast<long long>(nslots);
-  if (mp_aligned16(x) && mp_aligned16(y) && mp_aligned16(states) && x_pitch % PN == 0 && y_pitch % PN == 0 && channels % PN == 0 &&
+  if (mp_aligned16(x) && mp_aligned16(w) && (bias == nullptr || mp_aligned16(bias)) && mp_aligned16(y) && mp_aligned16(states) && x_pitch % PN == 0 && y_pitch % PN == 0 && channels % PN == 0 &&
       r * (channels / PN) <= 0x7fffffffll * 128)
     conv_token_run<T, PN>(xt, x_pitch, wt, bt, st, sl, yt, y_pitch, r, n, static_cast<int>(channels), static_cast<int>(width), ctx);
   else
@@ -375,7 +491,8 @@ void ssd_scan_token_impl(const void* x, len_t x_pitch, const void* dt_raw, len_t
   using A = typename Acc<T>::type;
   if (ngroups == 0 || heads % ngroups != 0) MP_FATAL("ssd_scan_token: heads %lu not divisible by groups %lu", heads, ngroups);
   if (x_pitch < heads * headdim || y_pitch < heads * headdim || bc_pitch < ngroups * dstate || dt_pitch < heads) MP_FATAL("ssd_scan_token: a row pitch is below its columns");
-  if (!fits(rows) || !fits(nslots) || !fits(heads * headdim) || !fits(headdim * dstate)) MP_FATAL("ssd_scan_token: rows, slots and sizes are counted in 31 bits");
+  if (!fits(rows) || !fits(nslots) || !fits(heads * headdim) || !fits(headdim * dstate) || dstate > 1ull << 30)
+    MP_FATAL("ssd_scan_token: rows, slots and sizes are counted in 31 bits");
   if (rows == 0 || heads == 0 || headdim == 0) return;
   if (dstate == 0) MP_FATAL("ssd_scan_token: no state");
   const int P = static_cast<int>(headdim), N = static_cast<int>(dstate);
@@ -383,20 +500,33 @@ void ssd_scan_token_impl(const void* x, len_t x_pitch, const void* dt_raw, len_t
   const int V = vec ? static_cast<int>(16 / sizeof(A)) : 1;
   int width = 1;
   while (width < 32 && width * V < N) width <<= 1;
-  // a warp has ST_U rows p for each of its lane groups; a CTA of up to four warps
-  const int rows_per_warp = ST_U * (32 / width), need = (P + rows_per_warp - 1) / rows_per_warp;
-  const long long units = static_cast<long long>(rows) * static_cast<long long>(heads);
-  const int warps = units >= 2ll * mp_sm_count(ctx) && need >= 4 ? 4 : need >= 2 && units >= mp_sm_count(ctx) ? 2 : 1;
+  // A warp has ST_U rows p for each of its lane groups at a time, twice where that leaves four warps for every scheduler; a CTA of up to four warps.
+  const int at_once = ST_U * (32 / width), turns = (P + at_once - 1) / at_once;
+  const long long units = static_cast<long long>(rows) * static_cast<long long>(heads), plenty = 16ll * mp_sm_count(ctx);
+  const int batches = turns > 1 && units * ((turns + 1) / 2) >= plenty ? 2 : 1;
+  const int need = (turns + batches - 1) / batches;
+  const int warps = units * need < 2ll * mp_sm_count(ctx) ? 1 : need >= 4 ? 4 : need >= 2 ? 2 : 1;
   const int splits = (need + warps - 1) / warps;
   if (units * splits > 0x7fffffffll) MP_FATAL("ssd_scan_token: %lu rows of %lu heads are too many for one launch", rows, heads);
   MpLaunch go(static_cast<unsigned>(units * splits), 32 * warps, 0, mp_stream(ctx));
   auto run = [&](auto kernel) {
     go(kernel, static_cast<const T*>(x), x_pitch, static_cast<const T*>(dt_raw), dt_pitch, static_cast<const A*>(dt_bias), static_cast<const A*>(A_log),
        static_cast<const T*>(Bm), static_cast<const T*>(Cm), bc_pitch, static_cast<A*>(states), static_cast<const int*>(slots), static_cast<T*>(y), y_pitch,
-       static_cast<long long>(nslots), static_cast<int>(heads), P, N, static_cast<int>(ngroups), width, splits);
+       static_cast<long long>(nslots), static_cast<int>(heads), P, N, static_cast<int>(ngroups), batches, splits);
   };
-  if (vec) run(scan_token_kernel<T, static_cast<int>(16 / sizeof(A))>);
-  else run(scan_token_kernel<T, 1>);
+  auto by_width = [&](auto vec_size) {
+    constexpr int VS = decltype(vec_size)::value;
+    switch (width) {
+      case 1: run(scan_token_kernel<T, VS, 1>); break;
+      case 2: run(scan_token_kernel<T, VS, 2>); break;
+      case 4: run(scan_token_kernel<T, VS, 4>); break;
+      case 8: run(scan_token_kernel<T, VS, 8>); break;
+      case 16: run(scan_token_kernel<T, VS, 16>); break;
+      default: run(scan_token_kernel<T, VS, 32>);
+    }
+  };
+  if (vec) by_width(std::integral_constant<int, static_cast<int>(16 / sizeof(A))>());
+  else by_width(std::integral_constant<int, 1>());
   MP_LAUNCH_CHECK();
 }
 
