@@ -13,20 +13,39 @@
 
 namespace {
 
-constexpr int BM_THREADS = 256, BM_WARPS = BM_THREADS / 32;
+constexpr int BM_THREADS = 128, BM_WARPS = BM_THREADS / 32;
 constexpr int BM_LIST = 32;
 constexpr int BM_HELD = 512;             // values on a CTA's list
 constexpr int BM_NONE = 0x7fffffff;      // token of an empty place
 constexpr int BM_MAX_BEAMS = 64;
 
-template <typename V> struct Entry { V v; int i; };
-template <typename V> __device__ __forceinline__ bool better(const Entry<V>& a, const Entry<V>& b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
-template <typename V> __device__ __forceinline__ Entry<V> entry_xor(const Entry<V>& e, int o) {
-  return {__shfl_xor_sync(0xffffffffu, e.v, o), __shfl_xor_sync(0xffffffffu, e.i, o)};
+// A value and its token (or beam and place) as whole numbers in the order of better-first: comparisons of floating point values in r64 take ten
+// times as long.  A value of 32 bits and its token make one number.  (-0 is taken for 0.)
+template <typename V> struct Entry;
+template <> struct Entry<float> { unsigned long long k; };
+template <> struct Entry<double> { long long v; int i; };
+__device__ __forceinline__ Entry<float> entry(float v, int i) {
+  const int bits = __float_as_int(v + 0.f);
+  const unsigned up = bits < 0 ? ~static_cast<unsigned>(bits) : static_cast<unsigned>(bits) | 0x80000000u;
+  return {static_cast<unsigned long long>(up) << 32 | static_cast<unsigned>(BM_NONE - i)};
 }
-template <typename V> __device__ __forceinline__ Entry<V> entry_at(const Entry<V>& e, int lane) {
-  return {__shfl_sync(0xffffffffu, e.v, lane), __shfl_sync(0xffffffffu, e.i, lane)};
+__device__ __forceinline__ Entry<double> entry(double v, int i) {
+  const long long bits = __double_as_longlong(v + 0.0);
+  return {bits < 0 ? bits ^ 0x7fffffffffffffffll : bits, i};
 }
+__device__ __forceinline__ float value_of(const Entry<float>& e) {
+  const unsigned up = static_cast<unsigned>(e.k >> 32);
+  return __int_as_float(static_cast<int>(up & 0x80000000u ? up & 0x7fffffffu : ~up));
+}
+__device__ __forceinline__ double value_of(const Entry<double>& e) { return __longlong_as_double(e.v < 0 ? e.v ^ 0x7fffffffffffffffll : e.v); }
+__device__ __forceinline__ int index_of(const Entry<float>& e) { return BM_NONE - static_cast<int>(static_cast<unsigned>(e.k)); }
+__device__ __forceinline__ int index_of(const Entry<double>& e) { return e.i; }
+__device__ __forceinline__ bool better(const Entry<float>& a, const Entry<float>& b) { return a.k > b.k; }
+__device__ __forceinline__ bool better(const Entry<double>& a, const Entry<double>& b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
+__device__ __forceinline__ Entry<float> entry_xor(const Entry<float>& e, int o) { return {__shfl_xor_sync(0xffffffffu, e.k, o)}; }
+__device__ __forceinline__ Entry<double> entry_xor(const Entry<double>& e, int o) { return {__shfl_xor_sync(0xffffffffu, e.v, o), __shfl_xor_sync(0xffffffffu, e.i, o)}; }
+__device__ __forceinline__ Entry<float> entry_at(const Entry<float>& e, int lane) { return {__shfl_sync(0xffffffffu, e.k, lane)}; }
+__device__ __forceinline__ Entry<double> entry_at(const Entry<double>& e, int lane) { return {__shfl_sync(0xffffffffu, e.v, lane), __shfl_sync(0xffffffffu, e.i, lane)}; }
 __device__ __forceinline__ float lowest(float) { return -INFINITY; }
 __device__ __forceinline__ double lowest(double) { return -INFINITY; }
 
@@ -35,7 +54,7 @@ template <typename V>
 __device__ __forceinline__ void merge_lists(Entry<V>& a, const Entry<V>& b, int lane) {
   const Entry<V> r = entry_at(b, 31 - lane);
   if (better(r, a)) a = r;               // now bitonic
-#pragma unroll
+#pragma unroll 1
   for (int o = 16; o > 0; o >>= 1) {
     const Entry<V> other = entry_xor(a, o);
     const bool upper = (lane & o) != 0;  // keeps the worse one
@@ -45,32 +64,40 @@ __device__ __forceinline__ void merge_lists(Entry<V>& a, const Entry<V>& b, int 
 // A warp's entries, best first.
 template <typename V>
 __device__ __forceinline__ void sort_list(Entry<V>& a, int lane) {
-#pragma unroll
+#pragma unroll 1
   for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
+#pragma unroll 1
     for (int o = size >> 1; o > 0; o >>= 1) {
       const Entry<V> other = entry_xor(a, o);
       const bool worse = ((lane & o) != 0) != ((lane & size) != 0);      // this lane keeps the worse one
       if (better(other, a) != worse) a = other;
     }
 }
-template <typename V>
-__device__ __forceinline__ V sort_values(V a, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1) {
-      const V other = __shfl_xor_sync(0xffffffffu, a, o);
-      const bool less = ((lane & o) != 0) != ((lane & size) != 0);
-      a = (other > a) != less ? other : a;
-    }
-  return a;
+// The warp's value at place `place` (0: the largest), counting equal ones.
+__device__ __forceinline__ float nth_largest(float v, int place) {
+  const int bits = __float_as_int(v);
+  int key = bits < 0 ? bits ^ 0x7fffffff : bits, most = key;      // whole numbers in the same order
+  for (int i = 0; i <= place; ++i) {
+    most = __reduce_max_sync(0xffffffffu, key);
+    const unsigned who = __ballot_sync(0xffffffffu, key == most);
+    if ((threadIdx.x & 31) == __ffs(who) - 1) key = 0x80000000;
+  }
+  return __int_as_float(most < 0 ? most ^ 0x7fffffff : most);
+}
+__device__ __forceinline__ double nth_largest(double v, int place) {
+  double most = v;
+  for (int i = 0; i <= place; ++i) {
+    most = warp_reduce<MaxOp>(v);
+    const unsigned who = __ballot_sync(0xffffffffu, v == most);
+    if ((threadIdx.x & 31) == __ffs(who) - 1) v = -INFINITY;
+  }
+  return most;
 }
 // `e` takes its place in the list.
 template <typename V>
 __device__ __forceinline__ void insert(Entry<V>& list, const Entry<V>& e, int lane) {
   const int at = __popc(__ballot_sync(0xffffffffu, better(list, e)));
-  const Entry<V> before = {__shfl_up_sync(0xffffffffu, list.v, 1), __shfl_up_sync(0xffffffffu, list.i, 1)};
+  const Entry<V> before = entry_at(list, lane > 0 ? lane - 1 : 0);
   if (lane == at) list = e;
   else if (lane > at) list = before;
 }
@@ -133,8 +160,7 @@ template <typename A>
 struct BeamScratch {     // per row and piece
   A* top;                // maximum
   double* sum;           // sum of exp(logit - maximum)
-  A* value;              // [32] best logits
-  int* token;            // [32] their tokens
+  Entry<A>* best;        // [32] best logits
 };
 template <typename A>
 __host__ __device__ inline BeamScratch<A> beam_carve(void* scratch, size_t pieces) {
@@ -142,97 +168,129 @@ __host__ __device__ inline BeamScratch<A> beam_carve(void* scratch, size_t piece
   unsigned char* p = static_cast<unsigned char*>(scratch);
   b.sum = reinterpret_cast<double*>(p); p += pieces * sizeof(double);
   b.top = reinterpret_cast<A*>(p); p += pieces * sizeof(double);
-  b.value = reinterpret_cast<A*>(p); p += pieces * BM_LIST * sizeof(A);
-  b.token = reinterpret_cast<int*>(p);
+  b.best = reinterpret_cast<Entry<A>*>(p);
   return b;
 }
-inline size_t beam_bytes(size_t pieces, size_t acc) { return pieces * (2 * sizeof(double) + BM_LIST * (acc + sizeof(int))); }
+template <typename A> inline size_t beam_bytes(size_t pieces) { return pieces * (2 * sizeof(double) + BM_LIST * sizeof(Entry<A>)); }
 
-// Pieces of a row: two packs for each thread of a CTA at least, four CTAs for every SM where the rows are too few.
+// Pieces of a row: two packs for each thread of a CTA at least, eight CTAs for every SM where the rows are too few.
 inline int beam_pieces(size_t rows, size_t vocab, size_t size) {
   const size_t most = (vocab * size + 2 * 16 * BM_THREADS - 1) / (2 * 16 * BM_THREADS);
-  size_t want = (4 * 148 + rows - 1) / rows;
+  size_t want = 8 * 148 / rows;
   if (want > most) want = most;
   return static_cast<int>(want < 1 ? 1 : want);
+}
+
+// Pack k (of `packs`) of a row that begins off the 16-byte boundary: two aligned words, moved together.  Its first and last pack, whose words reach
+// over the row's ends, are read value by value.
+template <typename T>
+__device__ __forceinline__ Pack<T> fetch_shifted(const T* src, int k, int packs) {
+  union { uint32_t w[8]; uint4 u[2]; Pack<T> p; } x;
+  const unsigned off = reinterpret_cast<uintptr_t>(src) & 15u;
+  if (k == 0 || k == packs - 1) {
+#pragma unroll
+    for (int e = 0; e < Pack<T>::N; ++e) x.p.v[e] = src[static_cast<size_t>(k) * Pack<T>::N + e];
+    return x.p;
+  }
+  const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(src) - off) + k;
+  x.u[0] = at[0];
+  x.u[1] = off != 0 ? at[1] : x.u[0];
+#pragma unroll
+  for (int e = 0; e < 6; ++e) x.w[e] = off & 8 ? x.w[e + 2] : x.w[e];
+#pragma unroll
+  for (int e = 0; e < 5; ++e) x.w[e] = off & 4 ? x.w[e + 1] : x.w[e];
+  if constexpr (sizeof(T) == 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.w[e] = __funnelshift_r(x.w[e], x.w[e + 1], off & 2 ? 16 : 0);
+  return x.p;
 }
 
 // A beam from which nothing goes on, or nothing but the end: its logits are not read.
 template <typename A> __device__ __forceinline__ bool beam_dead(A score) { return !(score > lowest(score)); }
 
-template <typename T>
-__global__ void __launch_bounds__(BM_THREADS) beam_rows_kernel(const T* __restrict__ logits, size_t pitch, const typename Acc<T>::type* __restrict__ scores,
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(BM_THREADS, sizeof(T) == 8 ? 6 : 8) beam_rows_kernel(const T* __restrict__ logits, size_t pitch, const typename Acc<T>::type* __restrict__ scores,
                                                                const int* __restrict__ finished, BeamScratch<typename Acc<T>::type> out, int vocab, int picks,
                                                                int pieces) {
   mp_grid_dependency();
   using A = typename Acc<T>::type;
-  constexpr int V = Pack<T>::N, U = 4;
-  __shared__ A s_value[BM_WARPS][BM_LIST], s_top[BM_WARPS];
+  constexpr int V = Pack<T>::N, U = WHOLE ? 8 : 4;
+  __shared__ A s_top[BM_WARPS];
   __shared__ double s_sum[BM_WARPS];
-  __shared__ int s_token[BM_WARPS][BM_LIST], s_count, s_which[BM_HELD];
-  __shared__ A s_bound[BM_WARPS], s_held[BM_HELD];
+  __shared__ int s_count;
+  __shared__ A s_bound[BM_WARPS];
+  __shared__ Entry<A> s_held[BM_HELD], s_best[BM_WARPS][BM_LIST];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x / pieces;
   const int piece = blockIdx.x % pieces;
   if (beam_dead(scores[row]) || (finished != nullptr && finished[row] != 0)) return;
   const T* src = logits + row * pitch;
-  // Which thread adds up which value goes by the token alone, not by the address: equal rows get equal sums, and their beams tie.  A row off the
-  // 16-byte boundary is read value by value.
-  const bool whole = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+  // Which thread adds up which value goes by the token alone, not by the address: equal rows get equal sums, and their beams tie.
   const int packs = vocab / V, tail = vocab - packs * V;
   const int each = (packs + pieces - 1) / pieces;
   const int first = min(piece * each, packs), end = min(first + each, packs);
 
   A top = most_negative<A>(), sums[2] = {A(0), A(0)};
-  // this thread's packs, U at a time: what(pack, token of its first value)
+  auto fetch = [&](int k) {
+    if constexpr (WHOLE) return ld_pack(src, k);
+    return fetch_shifted(src, k, packs);
+  };
+  // this thread's packs, U at a time: what(pack, its number)
   auto stream = [&](auto what) {
     for (int k0 = first + tid; k0 < end; k0 += BM_THREADS * U) {
       Pack<T> in[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = k0 + u * BM_THREADS;
-        if (k < end) {
-          if (whole) {
-            in[u] = ld_pack(src, k);
-          } else {
+      for (int u = 0; u < U; ++u)
+        if (k0 + u * BM_THREADS < end) in[u] = fetch(k0 + u * BM_THREADS);
 #pragma unroll
-            for (int e = 0; e < V; ++e) in[u].v[e] = src[static_cast<size_t>(k) * V + e];
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = k0 + u * BM_THREADS;
-        if (k < end) what(in[u], k * V);
-      }
+      for (int u = 0; u < U; ++u)
+        if (k0 + u * BM_THREADS < end) what(in[u], k0 + u * BM_THREADS);
     }
   };
+  // The sum is kept below a value that was the maximum once: it moves on only when the maximum is 32 above it (e^32 times any number of terms is
+  // far from the end of fp32), which a stream does once or twice.
+  A base = most_negative<A>();
   auto raise = [&](A most) {
-    if (most > top) {
-      const A f = below_exp(top - most);
+    top = most > top ? most : top;
+    if (most > base + A(32)) {
+      const A f = below_exp(base - most);
       sums[0] *= f;
       sums[1] *= f;
-      top = most;
+      base = most;
     }
   };
-  stream([&](const Pack<T>& in, int) {
-    raise(pack_most(in));
+  // the two packs with the largest maxima, and the largest maximum of the others
+  A most1 = lowest(A(0)), most2 = most1, most3 = most1;
+  int pack1 = 0, pack2 = 0;
+  stream([&](const Pack<T>& in, int k) {
+    const A m = pack_most(in);
+    if (m > most2) {
+      most3 = most2;
+      const bool first_now = m > most1;
+      most2 = first_now ? most1 : m;
+      pack2 = first_now ? pack1 : k;
+      most1 = first_now ? m : most1;
+      pack1 = first_now ? k : pack1;
+    } else {
+      most3 = m > most3 ? m : most3;
+    }
+    raise(m);
     A v[V];
     unpack(in, v);
 #pragma unroll
-    for (int e = 0; e < V; e += 2) add_exp2(sums, top, v[e], v[e + 1]);
+    for (int e = 0; e < V; e += 2) add_exp2(sums, base, v[e], v[e + 1]);
   });
   const int at_tail = packs * V + tid;      // fewer than a pack
   const bool has_tail = piece == 0 && tid < tail;
   if (has_tail) {
     const A v = mp_up(src[at_tail]);
     raise(v);
-    sums[0] += below_exp(v - top);
+    sums[0] += below_exp(v - base);
   }
   const A sum = sums[0] + sums[1];
   if (tid == 0) s_count = 0;
   {
-    const A sorted = sort_values(top, lane);
-    const A at = __shfl_sync(0xffffffffu, sorted, (picks + BM_WARPS - 1) / BM_WARPS - 1);
+    const A at = nth_largest(top, (picks + BM_WARPS - 1) / BM_WARPS - 1);
     if (lane == 0) s_bound[warp] = at;
   }
   __syncthreads();
@@ -243,27 +301,33 @@ __global__ void __launch_bounds__(BM_THREADS) beam_rows_kernel(const T* __restri
   auto take = [&](A v, int i) {
     if (v >= bound) {
       const int at = atomicAdd(&s_count, 1);
-      if (at < BM_HELD) { s_held[at] = v; s_which[at] = i; }
+      if (at < BM_HELD) s_held[at] = entry(v, i);
     }
   };
   if (!(top < bound)) {
-    stream([&](const Pack<T>& in, int i) {
-      if (pack_most(in) < bound) return;
+    auto look = [&](const Pack<T>& in, int k) {
       A v[V];
       unpack(in, v);
 #pragma unroll
-      for (int e = 0; e < V; ++e) take(v[e], i + e);
-    });
+      for (int e = 0; e < V; ++e) take(v[e], k * V + e);
+    };
+    if (most3 < bound) {
+      if (most1 >= bound) look(fetch(pack1), pack1);
+      if (most2 >= bound) look(fetch(pack2), pack2);
+    } else {
+      stream([&](const Pack<T>& in, int k) { if (!(pack_most(in) < bound)) look(in, k); });
+    }
     if (has_tail) take(mp_up(src[at_tail]), at_tail);
   }
   __syncthreads();
   const int count = s_count;
-  Entry<A> list = {lowest(A(0)), BM_NONE};
+  const Entry<A> none = entry(lowest(A(0)), BM_NONE);
+  Entry<A> list = none;
   if (count <= BM_HELD) {
     // warp w has places 32 w ..; mostly there is work for the first ones only
     for (int k = warp * 32; k < count; k += BM_THREADS) {
-      Entry<A> e = {lowest(A(0)), BM_NONE};
-      if (k + lane < count) e = {s_held[k + lane], s_which[k + lane]};
+      Entry<A> e = none;
+      if (k + lane < count) e = s_held[k + lane];
       sort_list(e, lane);
       merge_lists(list, e, lane);
     }
@@ -273,36 +337,33 @@ __global__ void __launch_bounds__(BM_THREADS) beam_rows_kernel(const T* __restri
       const int k = k0 + lane;
 #pragma unroll 1
       for (int e = 0; e < V; ++e) {
-        Entry<A> mine = {lowest(A(0)), BM_NONE};
-        if (k < end) mine = {mp_up(src[static_cast<size_t>(k) * V + e]), k * V + e};
+        Entry<A> mine = none;
+        if (k < end) mine = entry(mp_up(src[static_cast<size_t>(k) * V + e]), k * V + e);
         offer(list, last, mine, picks, lane);
       }
     }
-    Entry<A> mine = {lowest(A(0)), BM_NONE};
-    if (has_tail) mine = {mp_up(src[at_tail]), at_tail};
+    Entry<A> mine = none;
+    if (has_tail) mine = entry(mp_up(src[at_tail]), at_tail);
     offer(list, last, mine, picks, lane);
   }
   // the warp's sum, then the CTA's
   const A wtop = warp_reduce<MaxOp>(top);
-  const double wsum = warp_reduce<SumOp>(static_cast<double>(sum) * static_cast<double>(below_exp(top - wtop)));
-  s_value[warp][lane] = list.v;
-  s_token[warp][lane] = list.i;
+  const double wsum = warp_reduce<SumOp>(static_cast<double>(sum) * static_cast<double>(below_exp(base - wtop)));
+  s_best[warp][lane] = list;
   if (lane == 0) { s_top[warp] = wtop; s_sum[warp] = wsum; }
   __syncthreads();
   const int busy = count <= BM_HELD ? (count + 31) / 32 : BM_WARPS;      // warps that have something on their lists
   for (int half = BM_WARPS / 2; half > 0; half >>= 1) {
     if (half >= busy) continue;
     if (warp < half) {
-      merge_lists(list, Entry<A>{s_value[warp + half][lane], s_token[warp + half][lane]}, lane);
-      s_value[warp][lane] = list.v;
-      s_token[warp][lane] = list.i;
+      merge_lists(list, s_best[warp + half][lane], lane);
+      s_best[warp][lane] = list;
     }
     __syncthreads();
   }
   if (warp == 0) {
     const size_t at = static_cast<size_t>(row) * pieces + piece;
-    out.value[at * BM_LIST + lane] = list.v;
-    out.token[at * BM_LIST + lane] = list.i;
+    out.best[at * BM_LIST + lane] = list;
     const A t = s_top[lane % BM_WARPS], ct = warp_reduce<MaxOp>(t);
     const double cs = warp_reduce_width<SumOp, BM_WARPS>(s_sum[lane % BM_WARPS] * static_cast<double>(below_exp(t - ct)));
     if (lane == 0) { out.top[at] = ct; out.sum[at] = cs; }
@@ -316,102 +377,95 @@ template <typename A>
 __global__ void __launch_bounds__(BM_MERGE_WARPS * 32) beam_merge_kernel(BeamScratch<A> in, const A* scores, const int* finished, int eos, A* next_scores,
                                                                          int* parents, int* tokens, int* next_finished, int beams, int vocab, int picks,
                                                                          int pieces, int share, int seats) {
-  __shared__ A s_value[BM_MERGE_WARPS][BM_LIST];
-  __shared__ int s_from[BM_MERGE_WARPS][BM_LIST], s_key[BM_MERGE_WARPS][BM_LIST];
-  __shared__ double s_score[BM_MERGE_WARPS][BM_LIST];
+  __shared__ Entry<A> s_best[BM_MERGE_WARPS][BM_LIST];
+  __shared__ Entry<double> s_score[BM_MERGE_WARPS][BM_LIST];
   __shared__ int s_token[BM_MAX_BEAMS][BM_LIST], s_done[BM_MAX_BEAMS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t search = blockIdx.x;
   const int places = BM_LIST / seats, seat = lane / places, place = lane % places;
   const int beams_at_once = BM_MERGE_WARPS / share;
-  Entry<double> best = {lowest(0.0), BM_NONE};
+  const Entry<A> none = entry(lowest(A(0)), BM_NONE);
+  Entry<double> best = entry(lowest(0.0), BM_NONE);
   mp_grid_dependency();
   for (int b0 = 0; b0 < beams; b0 += beams_at_once) {
     const int beam = b0 + warp / share, part = warp % share;
     const bool live = beam < beams;
     const size_t row = search * beams + (live ? beam : 0);
-    const A had = scores[row];
-    const bool done = finished != nullptr && finished[row] != 0, dead = beam_dead(had);
-    Entry<A> list = {lowest(A(0)), BM_NONE};
+    // (what a beam that is not looked at has in its place is anything: it is not used)
+    Entry<A> list = none;
     A top = most_negative<A>();
     double sum = 0;
-    if (live && !dead && !done) {
-      for (int k0 = part * seats; k0 < pieces; k0 += share * seats) {
-        const int k = k0 + seat;
-        Entry<A> e = {lowest(A(0)), BM_NONE};
-        if (k < pieces) {
-          const size_t at = (row * pieces + k) * BM_LIST + place;
-          e = {in.value[at], in.token[at]};
-        }
-        if (seats > 1) sort_list(e, lane);
-        if (k0 == part * seats) list = e;
-        else merge_lists(list, e, lane);
+    const A had = scores[row];
+    const bool done = finished != nullptr && finished[row] != 0, dead = beam_dead(had);
+    if (part == 0) {      // the pieces' sums under one maximum
+      for (int k = lane; k < pieces; k += 32) {
+        const A t = in.top[row * pieces + k];
+        const double more = in.sum[row * pieces + k];
+        const A both = t > top ? t : top;
+        sum = sum * static_cast<double>(below_exp(top - both)) + more * static_cast<double>(below_exp(t - both));
+        top = both;
       }
-      if (part == 0) {      // the pieces' sums under one maximum
-        for (int k = lane; k < pieces; k += 32) {
-          const A t = in.top[row * pieces + k];
-          const double more = in.sum[row * pieces + k];
-          const A both = t > top ? t : top;
-          sum = sum * static_cast<double>(below_exp(top - both)) + more * static_cast<double>(below_exp(t - both));
-          top = both;
-        }
-        const A all = warp_reduce<MaxOp>(top);
-        sum = warp_reduce<SumOp>(sum * static_cast<double>(below_exp(top - all)));
-        top = all;
-      }
+    }
+    for (int k0 = part * seats; k0 < pieces; k0 += share * seats) {
+      const int k = k0 + seat;
+      Entry<A> e = none;
+      if (live && k < pieces) e = in.best[(row * pieces + k) * BM_LIST + place];
+      if (seats > 1) sort_list(e, lane);
+      merge_lists(list, e, lane);
+    }
+    if (part == 0) {
+      const A all = warp_reduce<MaxOp>(top);
+      sum = warp_reduce<SumOp>(sum * static_cast<double>(below_exp(top - all)));
+      top = all;
     }
     if (share > 1) {
       if (b0 != 0) __syncthreads();      // the lists of the beams before have been read
-      s_value[warp][lane] = list.v;
-      s_from[warp][lane] = list.i;
+      s_best[warp][lane] = list;
       __syncthreads();
       for (int half = share / 2; half > 0; half >>= 1) {
         if (part < half) {
-          merge_lists(list, Entry<A>{s_value[warp + half][lane], s_from[warp + half][lane]}, lane);
-          s_value[warp][lane] = list.v;
-          s_from[warp][lane] = list.i;
+          merge_lists(list, s_best[warp + half][lane], lane);
+          s_best[warp][lane] = list;
         }
         if (half > 1) __syncthreads();
       }
     }
     if (live && part == 0) {
       double score = lowest(0.0);
+      int token = lane;
       if (dead) {
-        list.i = lane;
+        // its tokens rank in their order
       } else if (done) {
-        list.i = lane == 0 ? eos : lane - 1 < eos ? lane - 1 : lane;
+        token = lane == 0 ? eos : lane - 1 < eos ? lane - 1 : lane;
         if (lane == 0) score = static_cast<double>(had);
       } else if (sum > 0 && sum < 1.0 / 0.0) {
-        score = static_cast<double>(had) + (static_cast<double>(list.v) - (static_cast<double>(top) + log(sum)));
+        score = static_cast<double>(had) + (static_cast<double>(value_of(list)) - (static_cast<double>(top) + log(sum)));
         if (score != score) score = lowest(0.0);      // an infinite score behind a token that is ruled out
-      } else {      // a NaN or an infinity among the logits, or nothing above minus infinity: no probabilities
-        list.i = lane;
-      }
-      s_token[beam][lane] = list.i;
+        token = index_of(list);
+      }      // else a NaN or an infinity among the logits, or nothing above minus infinity: no probabilities
+      s_token[beam][lane] = token;
       if (lane == 0) s_done[beam] = done;
       const bool wanted = lane < picks;
-      const Entry<double> e = {wanted ? score : lowest(0.0), wanted ? beam * BM_LIST + lane : BM_NONE};
+      const Entry<double> e = entry(wanted ? score : lowest(0.0), wanted ? beam * BM_LIST + lane : BM_NONE);
       if (b0 == 0) best = e;
       else merge_lists(best, e, lane);
     }
   }
   // the warps with beams: every `share`-th
-  s_score[warp][lane] = best.v;
-  s_key[warp][lane] = best.i;
+  s_score[warp][lane] = best;
   __syncthreads();
   for (int half = BM_MERGE_WARPS / 2; half >= share; half >>= 1) {
     if (half >= beams * share) continue;
     if (warp < half) {
-      merge_lists(best, Entry<double>{s_score[warp + half][lane], s_key[warp + half][lane]}, lane);
-      s_score[warp][lane] = best.v;
-      s_key[warp][lane] = best.i;
+      merge_lists(best, s_score[warp + half][lane], lane);
+      s_score[warp][lane] = best;
     }
     __syncthreads();
   }
   if (warp == 0 && lane < picks) {
     const size_t at = search * picks + lane;
-    const int beam = best.i / BM_LIST, token = s_token[beam][best.i % BM_LIST];
-    next_scores[at] = static_cast<A>(best.v);
+    const int key = index_of(best), beam = key / BM_LIST, token = s_token[beam][key % BM_LIST];
+    next_scores[at] = static_cast<A>(value_of(best));
     parents[at] = beam;
     tokens[at] = token;
     if (next_finished != nullptr) next_finished[at] = s_done[beam] != 0 || token == eos;
@@ -433,9 +487,10 @@ void beam_select_impl(const void* logits, len_t logits_pitch, const void* scores
   if (rows * pieces > 0x7fffffffull) MP_FATAL("beam_select: %lu searches are too many for one launch", batch);
   if (eos >= vocab) { finished = nullptr; next_finished = nullptr; }      // no end token
   const BeamScratch<A> sc = beam_carve<A>(scratch, rows * pieces);
+  const bool whole = mp_aligned16(logits) && logits_pitch % Pack<T>::N == 0;
   MpLaunch(static_cast<unsigned>(rows * pieces), BM_THREADS, 0, mp_stream(ctx))(
-      beam_rows_kernel<T>, static_cast<const T*>(logits), logits_pitch, static_cast<const A*>(scores), static_cast<const int*>(finished), sc,
-      static_cast<int>(vocab), static_cast<int>(picks), pieces);
+      whole ? beam_rows_kernel<T, true> : beam_rows_kernel<T, false>, static_cast<const T*>(logits), logits_pitch, static_cast<const A*>(scores),
+      static_cast<const int*>(finished), sc, static_cast<int>(vocab), static_cast<int>(picks), pieces);
   MP_LAUNCH_CHECK();
   int share = 1, seats = 1;
   while (share < BM_MERGE_WARPS && 2 * share * static_cast<int>(beams) <= BM_MERGE_WARPS && share < pieces) share <<= 1;
@@ -453,8 +508,8 @@ extern "C" len_t mpBeamSelectScratchBytes(uint32_t dtype_key, len_t batch, len_t
   (void)picks;
   const size_t rows = static_cast<size_t>(batch) * beams;
   if (rows == 0) return 256;
-  const size_t size = dtype_key == MP_R16 ? 2 : dtype_key == MP_R32 ? 4 : 8;
-  return static_cast<len_t>(beam_bytes(rows * beam_pieces(rows, vocab, size), dtype_key == MP_R64 ? 8 : 4) + 256);
+  const size_t size = dtype_key == MP_R16 ? 2 : dtype_key == MP_R32 ? 4 : 8, pieces = rows * beam_pieces(rows, vocab, size);
+  return static_cast<len_t>((dtype_key == MP_R64 ? beam_bytes<double>(pieces) : beam_bytes<float>(pieces)) + 256);
 }
 
 MP_STAMP3(beam_select,
