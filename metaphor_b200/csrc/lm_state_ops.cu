@@ -5,23 +5,6 @@
 
 namespace {
 
-template <typename T, int V>
-struct alignas(sizeof(T) * V) StVec { T v[V]; };
-
-template <typename T, int V>
-__device__ __forceinline__ void ld_vec(const T* p, typename Acc<T>::type* out) {
-  const StVec<T, V> x = *reinterpret_cast<const StVec<T, V>*>(p);
-#pragma unroll
-  for (int e = 0; e < V; ++e) out[e] = mp_up(x.v[e]);
-}
-template <typename T, int V>
-__device__ __forceinline__ void st_vec(T* p, const typename Acc<T>::type* in) {
-  StVec<T, V> x;
-#pragma unroll
-  for (int e = 0; e < V; ++e) x.v[e] = mp_down<T>(in[e]);
-  *reinterpret_cast<StVec<T, V>*>(p) = x;
-}
-
 // The taps of V neighbouring channels lie in a row: as many whole vectors as there are taps.
 template <typename T, int V, int W>
 __device__ __forceinline__ void load_taps(const T* __restrict__ w, int c, typename Acc<T>::type (&tap)[W][V]) {
@@ -32,59 +15,6 @@ __device__ __forceinline__ void load_taps(const T* __restrict__ w, int c, typena
   for (int k = 0; k < W; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) tap[k][e] = flat[e * W + k];
-}
-
-// out = a b + c, value by value; fp32 values two at a time.
-template <int V>
-__device__ __forceinline__ void fma_vec(float (&out)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
-  if constexpr (V % 2 == 0) {
-#pragma unroll
-    for (int e = 0; e < V; e += 2)
-      asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 c, a, b, c;\nmov.b64 {%0, %1}, c;\n}"
-          : "=f"(out[e]), "=f"(out[e + 1])
-          : "f"(a[e]), "f"(a[e + 1]), "f"(b[e]), "f"(b[e + 1]), "f"(c[e]), "f"(c[e + 1]));
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = a[e] * b[e] + c[e];
-  }
-}
-template <int V>
-__device__ __forceinline__ void fma_vec(double (&out)[V], const double (&a)[V], const double (&b)[V], const double (&c)[V]) {
-#pragma unroll
-  for (int e = 0; e < V; ++e) out[e] = a[e] * b[e] + c[e];
-}
-template <int V>
-__device__ __forceinline__ void mul_vec(float (&out)[V], const float (&a)[V], const float (&b)[V]) {
-  if constexpr (V % 2 == 0) {
-#pragma unroll
-    for (int e = 0; e < V; e += 2)
-      asm("{\n.reg .b64 c, a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 c, a, b;\nmov.b64 {%0, %1}, c;\n}"
-          : "=f"(out[e]), "=f"(out[e + 1])
-          : "f"(a[e]), "f"(a[e + 1]), "f"(b[e]), "f"(b[e + 1]));
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = a[e] * b[e];
-  }
-}
-template <int V>
-__device__ __forceinline__ void mul_vec(double (&out)[V], const double (&a)[V], const double (&b)[V]) {
-#pragma unroll
-  for (int e = 0; e < V; ++e) out[e] = a[e] * b[e];
-}
-template <typename T, int V>
-__device__ __forceinline__ void widen(const StVec<T, V>& x, typename Acc<T>::type (&out)[V]) {
-  if constexpr (std::is_same<T, __half>::value && V % 2 == 0) {
-    const __half2* h = reinterpret_cast<const __half2*>(x.v);
-#pragma unroll
-    for (int e = 0; e < V; e += 2) {
-      const float2 f = __half22float2(h[e / 2]);
-      out[e] = f.x;
-      out[e + 1] = f.y;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = mp_up(x.v[e]);
-  }
 }
 
 // pre * sigmoid(pre).  r16 results have 11 bits: the special-function unit's exponential and reciprocal (22 bits) lose nothing there.
@@ -268,28 +198,6 @@ __global__ void __launch_bounds__(128) conv_token_kernel(const T* x, size_t xp, 
 // ---------------------------------------------------------------------------
 constexpr int ST_U = 8;
 
-// The sum over the L lanes of a group of s[u]; returns that of row u = the lane's number in the group / (L / 8), for L < 8 that of row
-// u = lane * (8 / L) + k in s[k].
-template <int L, typename A>
-__device__ __forceinline__ void sum_rows(A (&s)[ST_U], int lane) {
-  int have = ST_U;
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    if (have > 1) {
-      have >>= 1;
-      const bool up = (lane & o) != 0;
-#pragma unroll
-      for (int k = 0; k < ST_U / 2; ++k)
-        if (k < have) {
-          const A send = up ? s[k] : s[k + have], keep = up ? s[k + have] : s[k];
-          s[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-        }
-    } else {
-      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
-    }
-  }
-}
-
 template <typename T, int V, int L>
 __global__ void __launch_bounds__(128, sizeof(T) == 8 ? 3 : 6) scan_token_kernel(const T* __restrict__ x, size_t xp, const T* __restrict__ raw, size_t rp,
                                                          const typename Acc<T>::type* __restrict__ dt_bias, const typename Acc<T>::type* __restrict__ A_log,
@@ -361,7 +269,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 8 ? 3 : 6) scan_token_kernel
         }
       }
     }
-    sum_rows<L>(sum, lane);
+    sum_rows<L, ST_U>(sum, lane);
     constexpr int HELD = L >= ST_U ? 1 : ST_U / L, SHARED = L >= ST_U ? L / ST_U : 1;      // sums of a lane, lanes with the same one
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {

@@ -50,3 +50,96 @@ template <> __device__ __forceinline__ double seq_exp<double>(double v) { return
 // softplus; where it is the identity to the last bit, it is taken for it
 __device__ __forceinline__ float seq_softplus(float v) { return v > 20.f ? v : log1pf(expf(v)); }
 __device__ __forceinline__ double seq_softplus(double v) { return v > 37.0 ? v : log1p(exp(v)); }
+
+// V neighbouring values.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) StVec { T v[V]; };
+
+template <typename T, int V>
+__device__ __forceinline__ void ld_vec(const T* p, typename Acc<T>::type* out) {
+  const StVec<T, V> x = *reinterpret_cast<const StVec<T, V>*>(p);
+#pragma unroll
+  for (int e = 0; e < V; ++e) out[e] = mp_up(x.v[e]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void st_vec(T* p, const typename Acc<T>::type* in) {
+  StVec<T, V> x;
+#pragma unroll
+  for (int e = 0; e < V; ++e) x.v[e] = mp_down<T>(in[e]);
+  *reinterpret_cast<StVec<T, V>*>(p) = x;
+}
+
+// out = a b + c, value by value; fp32 values two at a time.
+template <int V>
+__device__ __forceinline__ void fma_vec(float (&out)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2)
+      asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 c, a, b, c;\nmov.b64 {%0, %1}, c;\n}"
+          : "=f"(out[e]), "=f"(out[e + 1])
+          : "f"(a[e]), "f"(a[e + 1]), "f"(b[e]), "f"(b[e + 1]), "f"(c[e]), "f"(c[e + 1]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = a[e] * b[e] + c[e];
+  }
+}
+template <int V>
+__device__ __forceinline__ void fma_vec(double (&out)[V], const double (&a)[V], const double (&b)[V], const double (&c)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) out[e] = a[e] * b[e] + c[e];
+}
+template <int V>
+__device__ __forceinline__ void mul_vec(float (&out)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2)
+      asm("{\n.reg .b64 c, a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 c, a, b;\nmov.b64 {%0, %1}, c;\n}"
+          : "=f"(out[e]), "=f"(out[e + 1])
+          : "f"(a[e]), "f"(a[e + 1]), "f"(b[e]), "f"(b[e + 1]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = a[e] * b[e];
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_vec(double (&out)[V], const double (&a)[V], const double (&b)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) out[e] = a[e] * b[e];
+}
+template <typename T, int V>
+__device__ __forceinline__ void widen(const StVec<T, V>& x, typename Acc<T>::type (&out)[V]) {
+  if constexpr (std::is_same<T, __half>::value && V % 2 == 0) {
+    const __half2* h = reinterpret_cast<const __half2*>(x.v);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 f = __half22float2(h[e / 2]);
+      out[e] = f.x;
+      out[e + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = mp_up(x.v[e]);
+  }
+}
+
+// The sum over the L lanes of a group of s[u], U of them: a lane is left with that of u = its number in the group / (L / U), where
+// L < U with those of u = number * (U / L) + k in s[k].
+template <int L, int U, typename A>
+__device__ __forceinline__ void sum_rows(A (&s)[U], int lane) {
+  int have = U;
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) {
+    if (have > 1) {
+      have >>= 1;
+      const bool up = (lane & o) != 0;
+#pragma unroll
+      for (int k = 0; k < (U + 1) / 2; ++k)
+        if (k < have) {
+          const A send = up ? s[k] : s[k + have], keep = up ? s[k + have] : s[k];
+          s[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    } else {
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+    }
+  }
+}

@@ -144,34 +144,6 @@ struct ChunkArgs {
   uint32_t* status;
 };
 
-// Which steps a CTA has.  Ranges are numbered without a table: sequence s has the numbers from starts[s] / range + s on, which is at least as
-// many as it has ranges.
-struct Span { int s; long long lo, hi, seq_lo, seq_hi, slot; bool any; };
-__device__ __forceinline__ Span span_of(const ChunkArgs& a, int id) {
-  Span r;
-  if (a.range == 0) {
-    r.s = id;
-  } else {
-    const long long range = a.range;
-    r.s = warp_last_not_above(a.g.q.nseq - 1, id, [&](int i) { return seq_first(a.g.q, i) / range + i; });
-    if (r.s < 0) { r.s = 0; r.any = false; return r; }
-  }
-  r.seq_lo = seq_first(a.g.q, r.s);
-  r.seq_hi = seq_first(a.g.q, r.s + 1);
-  r.slot = seq_slot(a.g.q.slots, a.g.q.nslots, r.s);
-  if (a.range == 0) {
-    r.lo = r.seq_lo;
-    r.hi = r.seq_hi;
-    r.any = r.slot >= 0;
-  } else {
-    const long long j = id - (r.seq_lo / a.range + r.s);
-    r.lo = r.seq_lo + j * a.range;
-    r.hi = min(r.lo + a.range, r.seq_hi);
-    r.any = r.slot >= 0 && (r.lo < r.seq_hi || j == 0);
-  }
-  return r;
-}
-
 // A value that the compiler takes for a new one, so that what is made of it is made here and not kept in registers across the loop.
 __device__ __forceinline__ uint32_t fresh(uint32_t v) {
   asm volatile("" : "+r"(v));
@@ -367,7 +339,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
   mp_grid_wait();
   const int units = g.H * a.slices;
   const int id = blockIdx.x / units, unit = blockIdx.x % units, h = unit / a.slices, p0 = unit % a.slices * CP, grp = h / (g.H / g.G);
-  const Span sp = span_of(a, id);
+  const Span sp = span_of(a.g.q, a.range, id);
   if (!sp.any) { mp_launch_dependents(); return; }
   if (t.warp == 0) tmem_alloc(&tail->tmem, TM_COLS);
   const int pcols = min(CP, g.P - p0), length = static_cast<int>(sp.hi - sp.lo);
@@ -697,7 +669,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
   mp_grid_wait();
   const int units = g.H * a.slices;
   const int id = blockIdx.x / units, unit = blockIdx.x % units, h = unit / a.slices, p0 = unit % a.slices * CP, grp = h / (g.H / g.G);
-  const Span sp = span_of(a, id);
+  const Span sp = span_of(a.g.q, a.range, id);
   if (!sp.any || sp.hi >= sp.seq_hi) { mp_launch_dependents(); return; }      // nothing lies behind it
   if (t.warp == 0) tmem_alloc(&tail->tmem, CP);
   const int pcols = min(CP, g.P - p0);
