@@ -6,22 +6,24 @@
 namespace {
 
 // ---------------------------------------------------------------------------
-// The recurrence, step by step, for every type and shape.  Eight lanes have PV rows p of a state, each lane NV of their columns in registers, so
-// that nothing but B, C and x moves: they come through shared memory RT steps at a time, for the four warps of a CTA at once.  A step is three
-// operations for every value of the state (decay, product, sum over the columns), two values to an instruction in fp32: bound by the fp32 pipe.
+// The recurrence, step by step, for every type and shape.  LN lanes have PV rows p of a state, each lane NV of their columns in registers, so
+// that nothing but B, C and x moves: they come through shared memory RT steps at a time, for the four warps of a CTA at once, the next steps'
+// while these are worked on.  A step is three operations for every value of the state (decay, product, sum over the columns), two values to an
+// instruction in fp32: bound by the fp32 pipe.  A lane leaves its share of y_t in shared memory; the LN shares of a value are added up behind
+// the RT steps, so that no step waits for shuffles.  More lanes to a row make more and smaller CTAs; fewer rows to a lane would too, but then
+// B and C, of which a lane reads as many values as it has columns, would come from shared memory no faster than now for a quarter of the products.
 // Where the sequences and heads are too few for the GPU, long sequences are cut into ranges: first the states that all but the last ranges add
 // (`STATES`: from zero, without y), then carried from range to range, then the ranges side by side from the states that they receive.
 // ---------------------------------------------------------------------------
-constexpr int RC_LN = 8;
-
-template <typename T, int NV, int WARPS>
+template <typename T, int NP_, int LN>
 struct RecurrenceSizes {
   using A = typename Acc<T>::type;
-  static constexpr int PV = (sizeof(A) == 8 ? 2 : 4) / (NV > 16 ? 2 : 1);      // rows p of a lane: 64 registers of state
-  static constexpr int ROWS = PV * (32 / RC_LN);
-  static constexpr int NP = NV * RC_LN, THREADS = 32 * WARPS, PS = ROWS * WARPS;
+  static constexpr int NP = NP_, NV = NP / LN, PV = sizeof(A) == 8 ? 2 : 4;   // columns (padded) of a state and of a lane, rows of a lane
+  static constexpr int WARPS = 4, THREADS = 32 * WARPS;
+  static constexpr int ROWS = PV * (32 / LN), PS = ROWS * WARPS;               // rows p of a warp, of the CTA
   static constexpr int RT = sizeof(A) == 8 ? 8 : 16;                           // steps at a time
-  static constexpr size_t BYTES = sizeof(A) * (2 * RT * NP + RT * PS + 2 * RT);
+  static constexpr int TILE = 2 * RT * NP + RT * PS + 2 * RT;                  // B, C, x, decays, step sizes
+  static constexpr size_t BYTES = sizeof(A) * (2 * TILE + RT * THREADS * PV);  // two tiles, the lanes' shares of y
 };
 
 struct Ranges {
@@ -31,41 +33,46 @@ struct Ranges {
   bool packs;       // rows of x, B and C are whole 16-byte packs
 };
 
-// `rows` rows of NP values, 16 bytes at a time or one by one; zeros behind row `steps` and column `cols`.
+// RT rows of NP values, 16 bytes at a time or one by one; zeros behind row `steps` and column `cols`.  Values that need no conversion are copied
+// asynchronously.
 template <typename T, int NP, int RT, int THREADS>
 __device__ __forceinline__ void fetch_rows(typename Acc<T>::type* dst, const T* src, size_t pitch, int steps, int cols, bool packs) {
   using A = typename Acc<T>::type;
   constexpr int V = Pack<T>::N;
   if (packs && NP % V == 0) {
 #pragma unroll
-    for (int i = threadIdx.x; i < RT * NP / V; i += THREADS) {
-      const int t = i / (NP / V), n = i % (NP / V) * V;
-      A v[V] = {};
-      if (t < steps && n < cols) unpack(ld_pack(src + t * pitch + n, 0), v);
+    for (int k = 0; k < (RT * NP / V + THREADS - 1) / THREADS; ++k) {
+      const int i = threadIdx.x + k * THREADS, t = i / (NP / V), n = i % (NP / V) * V;
+      if (RT * NP / V % THREADS != 0 && i >= RT * NP / V) break;
+      const bool in = t < steps && n < cols;
+      const T* from = src + (in ? t * pitch + n : 0);
+      if constexpr (std::is_same<T, A>::value) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mp_smem_u32(dst + t * NP + n)), "l"(from), "r"(in ? 16 : 0) : "memory");
+      } else {
+        A v[V] = {};
+        if (in) unpack(ld_pack(from, 0), v);
 #pragma unroll
-      for (int e = 0; e < V; e += 16 / sizeof(A)) *reinterpret_cast<StVec<A, 16 / sizeof(A)>*>(dst + t * NP + n + e) = *reinterpret_cast<StVec<A, 16 / sizeof(A)>*>(v + e);
+        for (int e = 0; e < V; e += 16 / sizeof(A)) *reinterpret_cast<StVec<A, 16 / sizeof(A)>*>(dst + t * NP + n + e) = *reinterpret_cast<StVec<A, 16 / sizeof(A)>*>(v + e);
+      }
     }
   } else {
-#pragma unroll 8
-    for (int i = threadIdx.x; i < RT * NP; i += THREADS) {
-      const int t = i / NP, n = i % NP;
-      dst[i] = t < steps && n < cols ? mp_up(src[t * pitch + n]) : A(0);
+#pragma unroll
+    for (int k = 0; k < (RT * NP + THREADS - 1) / THREADS; ++k) {
+      const int i = threadIdx.x + k * THREADS, t = i / NP, n = i % NP;
+      if (RT * NP % THREADS == 0 || i < RT * NP) dst[i] = t < steps && n < cols ? mp_up(src[t * pitch + n]) : A(0);
     }
   }
 }
 
-template <typename T, int NV, int WARPS, bool STATES>
-__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_kernel(const PromptArgs g, const Ranges ranges, int splits) {
+template <typename T, int NP, int LN, bool STATES>
+__global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, const Ranges ranges, int splits) {
   mp_grid_dependency();
-  using Z = RecurrenceSizes<T, NV, WARPS>;
+  using Z = RecurrenceSizes<T, NP, LN>;
   using A = typename Z::A;
-  constexpr int NP = Z::NP, RT = Z::RT, PS = Z::PS, THREADS = Z::THREADS, PV = Z::PV, CV = 16 / sizeof(A);      // columns side by side
+  constexpr int NV = Z::NV, PV = Z::PV, RT = Z::RT, PS = Z::PS, THREADS = Z::THREADS, CV = 16 / sizeof(A);      // columns side by side
   extern __shared__ __align__(16) unsigned char rc_smem[];
-  A* sB = reinterpret_cast<A*>(rc_smem);      // [RT][NP], columns past N zero
-  A* sC = sB + RT * NP;
-  A* sx = sC + RT * NP;                       // [RT][PS]
-  A* sa = sx + RT * PS;                       // [RT]: decay
-  A* sdt = sa + RT;                           // [RT]: step size
+  // a tile: B [RT][NP], columns past N zero; C the same; x [RT][PS]; decays [RT]; step sizes [RT]
+  A* shares = reinterpret_cast<A*>(rc_smem) + 2 * Z::TILE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x % splits, idh = blockIdx.x / splits, h = idh % g.H, grp = h / (g.H / g.G);
   const Span sp = span_of(g.q, ranges.steps, idh / g.H);
@@ -76,74 +83,118 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_kernel(cons
   const T* Cm = static_cast<const T*>(g.Cm) + static_cast<size_t>(grp) * g.N;
   T* y = static_cast<T*>(g.y) + static_cast<size_t>(h) * g.P;
   const A bias = static_cast<const A*>(g.dt_bias)[h], rate = -seq_exp(static_cast<const A*>(g.A_log)[h]);
-  const int pg = lane / RC_LN, nl = lane % RC_LN;
+  const int pg = lane / LN, nl = lane % LN;
   const int pl = warp * Z::ROWS + pg * PV, p0 = split * PS + pl;     // this lane's first row, in the CTA and in the head
   A* state = static_cast<A*>(g.states) + (sp.slot * g.H + h) * static_cast<long long>(g.P) * g.N;
   A* local = static_cast<A*>(ranges.local) + static_cast<size_t>(idh) * g.P * g.N;
-  // a lane's columns are neighbours CV at a time: 16-byte reads of B and C, the eight lanes next to each other
+  // a lane's columns are neighbours CV at a time: 16-byte reads of B and C, the lanes of a row next to each other
   A S[PV][NV / CV][CV];
-  auto column = [&](int i, int e) { return (i * RC_LN + nl) * CV + e; };
+  auto column = [&](int i, int e) { return (i * LN + nl) * CV + e; };
   const bool received = !STATES && ranges.steps != 0 && sp.lo > sp.seq_lo, any = received || (!STATES && seq_resumes(g.q, sp.s));
   const A* from = received ? local : state;
+  const bool vectors = g.N % CV == 0 && mp_aligned16(g.states);
 #pragma unroll
   for (int p = 0; p < PV; ++p)
 #pragma unroll
-    for (int i = 0; i < NV / CV; ++i)
+    for (int i = 0; i < NV / CV; ++i) {
+      const A* at = from + static_cast<size_t>(p0 + p) * g.N + column(i, 0);
+      StVec<A, CV> v = {};
+      if (any && p0 + p < g.P) {
+        if (vectors) {
+          if (column(i, 0) < g.N) v = *reinterpret_cast<const StVec<A, CV>*>(at);
+        } else {
 #pragma unroll
-      for (int e = 0; e < CV; ++e) S[p][i][e] = any && p0 + p < g.P && column(i, e) < g.N ? from[static_cast<size_t>(p0 + p) * g.N + column(i, e)] : A(0);
-
-  A left = A(1);
-  for (long long t0 = sp.lo; t0 < sp.hi; t0 += RT) {
-    const int steps = sp.hi - t0 < RT ? static_cast<int>(sp.hi - t0) : RT;
-    __syncthreads();
-    fetch_rows<T, NP, RT, THREADS>(sB, Bm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
-    if (!STATES) fetch_rows<T, NP, RT, THREADS>(sC, Cm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
-    fetch_rows<T, PS, RT, THREADS>(sx, x + t0 * g.xp, g.xp, steps, g.P - split * PS, ranges.packs);
-    if (tid < RT) {
-      const A dt = tid < steps ? seq_softplus(mp_up(raw[(t0 + tid) * g.rp]) + bias) : A(0);
-      sdt[tid] = dt;
-      sa[tid] = seq_exp(dt * rate);
-    }
-    __syncthreads();
-    T* out = y + t0 * g.yp + p0;
-#pragma unroll 1
-    for (int t = 0; t < steps; ++t) {
-      A a[CV], xd[PV][CV], sum[PV][CV];
-      const A dt = sdt[t], a1 = sa[t];
-      if (STATES) left *= a1;
-#pragma unroll
-      for (int e = 0; e < CV; ++e) a[e] = a1;
-#pragma unroll
-      for (int p = 0; p < PV; ++p) {
-        const A v = dt * sx[t * PS + pl + p];
-#pragma unroll
-        for (int e = 0; e < CV; ++e) { xd[p][e] = v; sum[p][e] = A(0); }
+          for (int e = 0; e < CV; ++e)
+            if (column(i, e) < g.N) v.v[e] = at[e];
+        }
       }
 #pragma unroll
-      for (int i = 0; i < NV / CV; ++i) {
-        const StVec<A, CV> b = *reinterpret_cast<const StVec<A, CV>*>(sB + t * NP + column(i, 0));
-        StVec<A, CV> c;
-        if (!STATES) c = *reinterpret_cast<const StVec<A, CV>*>(sC + t * NP + column(i, 0));
+      for (int e = 0; e < CV; ++e) S[p][i][e] = v.v[e];
+    }
+
+  // (raw step sizes are asked for a tile earlier: one warp would wait for them, and all others for it)
+  auto raw_at = [&](long long t0) { return tid < RT && t0 + tid < sp.hi ? mp_up(raw[(t0 + tid) * g.rp]) : A(0); };
+  A raw_here = raw_at(sp.lo);
+  auto fetch = [&](long long t0) {
+    A* tile = reinterpret_cast<A*>(rc_smem) + ((t0 - sp.lo) / RT & 1) * Z::TILE;
+    const int steps = sp.hi - t0 < RT ? static_cast<int>(sp.hi - t0) : RT;
+    fetch_rows<T, NP, RT, THREADS>(tile, Bm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
+    if (!STATES) fetch_rows<T, NP, RT, THREADS>(tile + RT * NP, Cm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
+    fetch_rows<T, PS, RT, THREADS>(tile + 2 * RT * NP, x + t0 * g.xp, g.xp, steps, g.P - split * PS, ranges.packs);
+    if (tid < RT) {
+      const A dt = tid < steps ? seq_softplus(raw_here + bias) : A(0);
+      raw_here = raw_at(t0 + RT);
+      tile[2 * RT * NP + RT * PS + tid] = seq_exp(dt * rate);
+      tile[2 * RT * NP + RT * PS + RT + tid] = dt;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  A left = A(1);
+  if (sp.lo < sp.hi) fetch(sp.lo);
+  for (long long t0 = sp.lo; t0 < sp.hi; t0 += RT) {
+    const int steps = sp.hi - t0 < RT ? static_cast<int>(sp.hi - t0) : RT;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    if (t0 + RT < sp.hi) fetch(t0 + RT);
+    const A* sB = reinterpret_cast<const A*>(rc_smem) + ((t0 - sp.lo) / RT & 1) * Z::TILE;
+    const A *sC = sB + RT * NP, *sx = sC + RT * NP, *sa = sx + RT * PS, *sdt = sa + RT;
+    // UN steps at a time, so that one's operands are read and its sums finished beside another one's products; steps behind the last have a size
+    // of zero and change nothing.  (The shares are stored behind all of them: no read of a tile may pass a store.)
+    constexpr int UN = NV <= 4 ? 4 : 2;
+    for (int tu = 0; tu < steps; tu += UN) {
+      StVec<A, PV> total[UN];
+#pragma unroll
+      for (int q = 0; q < UN; ++q) {
+        const int t = tu + q;
+        A a[CV], xd[PV][CV], sum[PV][CV];
+        const A dt = sdt[t], a1 = sa[t];
+        if (STATES) left *= a1;
+#pragma unroll
+        for (int e = 0; e < CV; ++e) a[e] = a1;
 #pragma unroll
         for (int p = 0; p < PV; ++p) {
-          mul_vec(S[p][i], a, S[p][i]);
-          fma_vec(S[p][i], xd[p], b.v, S[p][i]);
-          if (!STATES) fma_vec(sum[p], c.v, S[p][i], sum[p]);
+          const A v = dt * sx[t * PS + pl + p];
+#pragma unroll
+          for (int e = 0; e < CV; ++e) { xd[p][e] = v; sum[p][e] = A(0); }
+        }
+#pragma unroll
+        for (int i = 0; i < NV / CV; ++i) {
+          const StVec<A, CV> b = *reinterpret_cast<const StVec<A, CV>*>(sB + t * NP + column(i, 0));
+          StVec<A, CV> c;
+          if (!STATES) c = *reinterpret_cast<const StVec<A, CV>*>(sC + t * NP + column(i, 0));
+#pragma unroll
+          for (int p = 0; p < PV; ++p) {
+            mul_vec(S[p][i], a, S[p][i]);
+            fma_vec(S[p][i], xd[p], b.v, S[p][i]);
+            if (!STATES) fma_vec(sum[p], c.v, S[p][i], sum[p]);
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < PV; ++p) {
+          total[q].v[p] = sum[p][0];
+#pragma unroll
+          for (int e = 1; e < CV; ++e) total[q].v[p] += sum[p][e];
         }
       }
       if (!STATES) {
-        A total[PV];
 #pragma unroll
-        for (int p = 0; p < PV; ++p) {
-          total[p] = sum[p][0];
-#pragma unroll
-          for (int e = 1; e < CV; ++e) total[p] += sum[p][e];
-        }
-        sum_rows<RC_LN, PV>(total, nl);
-        constexpr int SHARED = RC_LN / PV;      // lanes with the same sum
-        if (nl % SHARED == 0 && p0 + nl / SHARED < g.P) out[nl / SHARED] = mp_down<T>(total[0]);
-        out += g.yp;
+        for (int q = 0; q < UN; ++q) *reinterpret_cast<StVec<A, PV>*>(shares + ((tu + q) * THREADS + tid) * PV) = total[q];
       }
+    }
+    if (!STATES) {
+      __syncwarp();
+      // a lane has one of the warp's ROWS values of every (32 / ROWS)-th step; it begins with another one of the shares than its
+      // neighbours, which would all wait for the same bank
+      const int row = lane % Z::ROWS, first = lane / PV;
+      const A* at = shares + (warp * 32 + row / PV * LN) * PV + row % PV;
+      const int p = split * PS + warp * Z::ROWS + row;
+      for (int t = lane / Z::ROWS; t < steps; t += 32 / Z::ROWS) {
+        A v = A(0);
+#pragma unroll
+        for (int k = 0; k < LN; ++k) v += at[(t * THREADS + (first + k) % LN) * PV];
+        if (p < g.P) y[(t0 + t) * g.yp + p] = mp_down<T>(v);
+      }
+      __syncwarp();
     }
   }
   A* to = STATES ? local : state;
@@ -151,10 +202,21 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_kernel(cons
 #pragma unroll
   for (int p = 0; p < PV; ++p)
 #pragma unroll
-    for (int i = 0; i < NV / CV; ++i)
+    for (int i = 0; i < NV / CV; ++i) {
+      A* at = to + static_cast<size_t>(p0 + p) * g.N + column(i, 0);
+      StVec<A, CV> v;
 #pragma unroll
-      for (int e = 0; e < CV; ++e)
-        if (p0 + p < g.P && column(i, e) < g.N) to[static_cast<size_t>(p0 + p) * g.N + column(i, e)] = S[p][i][e];
+      for (int e = 0; e < CV; ++e) v.v[e] = S[p][i][e];
+      if (p0 + p < g.P) {
+        if (vectors) {
+          if (column(i, 0) < g.N) *reinterpret_cast<StVec<A, CV>*>(at) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < CV; ++e)
+            if (column(i, e) < g.N) at[e] = v.v[e];
+        }
+      }
+    }
   if (STATES && split == 0 && tid == 0) static_cast<A*>(ranges.decay)[idh] = left;
 }
 
@@ -195,69 +257,65 @@ __global__ void __launch_bounds__(256) recurrence_carry_kernel(const PromptArgs 
   }
 }
 
-// Steps of a range, 0 for whole sequences.  The host knows how many sequences and rows there are, not how long each is.  `units`: CTAs for one
-// sequence.  Two CTAs on each of 148 SMs keep the fp32 pipe fed: from there on whole sequences, since a range's state is made twice.  Otherwise
-// four CTAs for each SM, of 32 steps at least (one CTA takes them in about the time of the launches).
-int recurrence_range(size_t nseq, size_t rows, size_t units) {
-  if (nseq * units >= 2 * 148) return 0;
-  const size_t want = 4 * 148 / units + 1;
-  size_t range = ((rows + want - 1) / want + 15) / 16 * 16;
-  if (range < 32) range = 32;
-  return range >= rows ? 0 : static_cast<int>(range);
+// How a call is cut up.  The host knows how many sequences and rows there are, not how long each is.
+struct Cut { int lanes, splits, steps; size_t ids; };      // lanes of a row; CTAs of a head; steps of a range (0: whole sequences); ranges or sequences
+// `least`, `most`: lanes of a row; `held`: rows p of a lane.  Ranges of 64 steps or more where a sequence may be long and there are not twice as many
+// CTAs as the GPU holds (four for each of 148 SMs) all the same: a range's state is made twice.  Rows get more lanes where a head is small, or
+// where there are too few CTAs.
+Cut recurrence_cut(size_t nseq, size_t rows, size_t heads, size_t headdim, int held, int least, int most) {
+  Cut c{least, 0, 0, nseq};
+  auto rows_of = [&] { return static_cast<size_t>(held) * (128 / c.lanes); };
+  auto splits = [&] { return (headdim + rows_of() - 1) / rows_of(); };
+  while (c.lanes < most && 2 * headdim <= rows_of()) c.lanes <<= 1;
+  const size_t units = heads * splits(), longest = 2 * rows / nseq < rows ? 2 * rows / nseq : rows;      // (a guess)
+  if (nseq * units < 8 * 148 && longest > 320) {
+    const size_t want = 8 * 148 / units + 1;
+    size_t range = ((rows + want - 1) / want + 15) / 16 * 16;
+    if (range < 64) range = 64;
+    if (range < rows) { c.steps = static_cast<int>(range); c.ids = rows / range + nseq; }
+  }
+  while (c.lanes < most && c.ids * heads * splits() < 2 * 148) c.lanes <<= 1;
+  c.splits = static_cast<int>(splits());
+  return c;
 }
-size_t recurrence_ids(size_t nseq, size_t rows, int range) { return range == 0 ? nseq : rows / range + nseq; }
 
-template <typename T, int NV>
-int recurrence_warps(size_t headdim) {
-  constexpr size_t ROWS = RecurrenceSizes<T, NV, 1>::ROWS;
-  return headdim > 2 * ROWS ? 4 : headdim > ROWS ? 2 : 1;
-}
-template <typename T, int NV>
-size_t recurrence_splits(size_t headdim) {
-  const size_t rows = static_cast<size_t>(RecurrenceSizes<T, NV, 1>::ROWS) * recurrence_warps<T, NV>(headdim);
-  return (headdim + rows - 1) / rows;
-}
-
-template <typename T, int NV, int WARPS>
-void recurrence_run(const PromptArgs& g, const Ranges& r, StreamContext ctx) {
-  using Z = RecurrenceSizes<T, NV, WARPS>;
+template <typename T, int NP, int LN>
+void recurrence_run(const PromptArgs& g, const Ranges& r, const Cut& c, StreamContext ctx) {
+  using Z = RecurrenceSizes<T, NP, LN>;
   using A = typename Z::A;
-  const int splits = static_cast<int>(recurrence_splits<T, NV>(g.P));
-  const size_t ctas = recurrence_ids(g.q.nseq, g.q.rows, r.steps) * g.H * splits;
+  const size_t ctas = c.ids * g.H * c.splits;
   if (ctas > 0x7fffffffull) MP_FATAL("ssd_scan_prompt: too many sequences and heads for one launch");
   auto go = [&](auto kernel) {
     if (Z::BYTES > 48 * 1024) MP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Z::BYTES)));
-    MpLaunch(static_cast<unsigned>(ctas), Z::THREADS, Z::BYTES, mp_stream(ctx))(kernel, g, r, splits);
+    MpLaunch(static_cast<unsigned>(ctas), Z::THREADS, Z::BYTES, mp_stream(ctx))(kernel, g, r, c.splits);
     MP_LAUNCH_CHECK();
   };
   if (r.steps != 0) {
-    go(recurrence_kernel<T, NV, WARPS, true>);
+    go(recurrence_kernel<T, NP, LN, true>);
     const size_t parts = (static_cast<size_t>(g.P) * g.N + 255) / 256, carries = static_cast<size_t>(g.q.nseq) * g.H * parts;
     if (carries > 0x7fffffffull) MP_FATAL("ssd_scan_prompt: too many sequences and heads for one launch");
     MpLaunch(static_cast<unsigned>(carries), 256, 0, mp_stream(ctx))(recurrence_carry_kernel<A>, g, r, static_cast<int>(parts));
     MP_LAUNCH_CHECK();
   }
-  go(recurrence_kernel<T, NV, WARPS, false>);
+  go(recurrence_kernel<T, NP, LN, false>);
 }
 
-// what(columns of a lane)
+// what(padded columns, least and most lanes of a row): a lane has 4 to 16 columns
 template <typename F>
 auto by_columns(size_t dstate, F what) {
-  if (dstate <= 32) return what(std::integral_constant<int, 4>());
-  if (dstate <= 64) return what(std::integral_constant<int, 8>());
-  if (dstate <= 128) return what(std::integral_constant<int, 16>());
-  return what(std::integral_constant<int, 32>());
+  using std::integral_constant;
+  if (dstate <= 32) return what(integral_constant<int, 32>(), integral_constant<int, 8>(), integral_constant<int, 8>());
+  if (dstate <= 64) return what(integral_constant<int, 64>(), integral_constant<int, 8>(), integral_constant<int, 16>());
+  if (dstate <= 128) return what(integral_constant<int, 128>(), integral_constant<int, 8>(), integral_constant<int, 32>());
+  return what(integral_constant<int, 256>(), integral_constant<int, 16>(), integral_constant<int, 32>());
 }
+template <typename T> constexpr int recurrence_held = RecurrenceSizes<T, 32, 8>::PV;
 
-template <typename T>
-int recurrence_steps(size_t nseq, size_t rows, size_t heads, size_t headdim, size_t dstate) {
-  return by_columns(dstate, [&](auto nv) { return recurrence_range(nseq, rows, heads * recurrence_splits<T, decltype(nv)::value>(headdim)); });
-}
 template <typename T>
 size_t recurrence_scratch(size_t nseq, size_t rows, size_t heads, size_t headdim, size_t dstate) {
   if (nseq == 0 || heads == 0 || headdim == 0 || dstate == 0 || dstate > 256) return 256;
-  const int range = recurrence_steps<T>(nseq, rows, heads, headdim, dstate);
-  return range == 0 ? 256 : recurrence_ids(nseq, rows, range) * heads * (headdim * dstate + 1) * sizeof(typename Acc<T>::type) + 256;
+  const Cut c = by_columns(dstate, [&](auto, auto least, auto most) { return recurrence_cut(nseq, rows, heads, headdim, recurrence_held<T>, least.value, most.value); });
+  return c.steps == 0 ? 256 : c.ids * heads * (headdim * dstate + 1) * sizeof(typename Acc<T>::type) + 256;
 }
 
 template <typename T>
@@ -265,17 +323,21 @@ void recurrence(const PromptArgs& g, void* scratch, StreamContext ctx) {
   using A = typename Acc<T>::type;
   constexpr size_t V = Pack<T>::N;
   Ranges r{nullptr, nullptr, 0, g.P % V == 0 && g.N % V == 0 && g.xp % V == 0 && g.bcp % V == 0 && mp_aligned16(g.x) && mp_aligned16(g.Bm) && mp_aligned16(g.Cm)};
-  if (scratch != nullptr) {
-    r.steps = recurrence_steps<T>(g.q.nseq, g.q.rows, g.H, g.P, g.N);
-    r.local = scratch;
-    r.decay = static_cast<A*>(scratch) + recurrence_ids(g.q.nseq, g.q.rows, r.steps) * g.H * static_cast<size_t>(g.P) * g.N;
-  }
-  by_columns(g.N, [&](auto nv) {
-    constexpr int NV = decltype(nv)::value;
-    const int warps = recurrence_warps<T, NV>(g.P);
-    if (warps == 4) recurrence_run<T, NV, 4>(g, r, ctx);
-    else if (warps == 2) recurrence_run<T, NV, 2>(g, r, ctx);
-    else recurrence_run<T, NV, 1>(g, r, ctx);
+  by_columns(g.N, [&](auto np, auto least, auto most) {
+    constexpr int NP = decltype(np)::value, LEAST = decltype(least)::value, MOST = decltype(most)::value;
+    const size_t nseq = g.q.nseq, heads = g.H;
+    // (without scratch: whole sequences, as if there were no rows to cut)
+    const Cut c = recurrence_cut(nseq, scratch != nullptr ? g.q.rows : 0, heads, g.P, recurrence_held<T>, LEAST, MOST);
+    if (c.steps != 0) {
+      r.steps = c.steps;
+      r.local = scratch;
+      r.decay = static_cast<A*>(scratch) + c.ids * heads * static_cast<size_t>(g.P) * g.N;
+    }
+    if constexpr (LEAST <= 8)
+      if (c.lanes == 8) return recurrence_run<T, NP, 8>(g, r, c, ctx);
+    if constexpr (MOST >= 16)
+      if (c.lanes == 16) return recurrence_run<T, NP, 16>(g, r, c, ctx);
+    if constexpr (MOST >= 32) recurrence_run<T, NP, 32>(g, r, c, ctx);
   });
 }
 
