@@ -282,7 +282,7 @@ MP_DECL3(inner_product_bji_bjk_bik, const void* a_data, const void* b_data, cons
  * batch can be padded.  No two sequences of a call have the same slot (of two that had, one or the other's results would stay).
  * A prompt goes on from its state where resume[i] != 0 (int32) and begins with zeros elsewhere (resume NULL: everywhere);
  * a token always goes on.  The state behind the last row replaces the one before.  starts, slots and resume are DEVICE arrays.
- * Rows of y that belong to no sequence keep what they hold.  Prompt forms: y does not overlap the inputs. */
+ * Rows of y that belong to no sequence keep what they hold.  y does not overlap the inputs, except where said. */
 
 /* launch_causal_conv1d_silu that begins with the last width - 1 inputs of each sequence.
  * states: T [nslots, width - 1, channels], the oldest input first; w, bias as there.  Token form: y may be x. */
@@ -292,7 +292,8 @@ MP_DECL3(causal_conv1d_silu_token, const void* x, len_t x_pitch, const void* w, 
  *   dt = softplus(dt_raw + dt_bias[h]),  S_t = exp(-dt_t exp(A_log[h])) S_{t-1} + dt_t x_t (x) B_t,  y_t = S_t C_t.
  * x, y: rows of heads * headdim elements, B, C: rows of ngroups * dstate, dt_raw: rows of heads, all of T with row pitches of
  * their own (B and C share one); dt_bias, A_log: acc [heads]; states: acc [nslots, heads, headdim, dstate].  dstate is 256
- * at most in the prompt form.  Prompt scratch: mpSsdScanPromptScratchBytes(...) bytes owned by the caller, 16-byte aligned. */
+ * at most in the prompt form.  Prompt scratch: mpSsdScanPromptScratchBytes(...) bytes owned by the caller, 16-byte aligned; NULL: long
+ * sequences are not cut into ranges that run side by side. */
 MP_DECL3(ssd_scan_prompt, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, const void* resume, const void* starts, void* y, len_t y_pitch, void* scratch, len_t nseq, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
 MP_DECL3(ssd_scan_token, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, void* y, len_t y_pitch, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
 MP_EXTERN_C len_t mpSsdScanPromptScratchBytes(uint32_t dtype_key, len_t nseq, len_t rows, len_t heads, len_t headdim, len_t dstate, len_t ngroups);

@@ -247,12 +247,12 @@ __global__ void __launch_bounds__(BM_THREADS, sizeof(T) == 8 ? 6 : 8) beam_rows_
         if (k0 + u * BM_THREADS < end) what(in[u], k0 + u * BM_THREADS);
     }
   };
-  // The sum is kept below a value that was the maximum once: it moves on only when the maximum is 32 above it (e^32 times any number of terms is
-  // far from the end of fp32), which a stream does once or twice.
+  // The sum is kept relative to a value that was the maximum once: it moves on only when the maximum is more than 4 above it (the exponents'
+  // rounding grows with the distance: 4 half steps at 4), which a stream does a few times.
   A base = most_negative<A>();
   auto raise = [&](A most) {
     top = most > top ? most : top;
-    if (most > base + A(32)) {
+    if (most > base + A(4)) {
       const A f = below_exp(base - most);
       sums[0] *= f;
       sums[1] *= f;

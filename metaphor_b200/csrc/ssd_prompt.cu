@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, 
     if (tid < RT) {
       const A dt = tid < steps ? seq_softplus(raw_here + bias) : A(0);
       raw_here = raw_at(t0 + RT);
-      tile[2 * RT * NP + RT * PS + tid] = seq_exp(dt * rate);
+      tile[2 * RT * NP + RT * PS + tid] = tid < steps ? seq_exp(dt * rate) : A(1);
       tile[2 * RT * NP + RT * PS + RT + tid] = dt;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -166,6 +166,10 @@ __global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, 
           for (int p = 0; p < PV; ++p) {
             mul_vec(S[p][i], a, S[p][i]);
             fma_vec(S[p][i], xd[p], b.v, S[p][i]);
+            if ((i + 1) * LN * CV > g.N) {      // columns behind the last stay zero: an infinity times nothing would reach y
+#pragma unroll
+              for (int e = 0; e < CV; ++e) S[p][i][e] = column(i, e) < g.N ? S[p][i][e] : A(0);
+            }
             if (!STATES) fma_vec(sum[p], c.v, S[p][i], sum[p]);
           }
         }

@@ -273,7 +273,7 @@ __device__ __forceinline__ void add_state(f2 (&S)[16], uint32_t tmem, float tota
 // A chunk step by step, for values that the products would spread.  S lies where the operands' terms were, [64 p][128 n]; a thread has column
 // n = row, 32 rows p.  y_p is summed over a warp's 32 columns lane against lane, then over the warps in turn.  OUT: with y.
 template <bool OUT>
-__device__ __forceinline__ void chunk_plain(unsigned char* smem, ChunkTail* tail, const Lane& t, f2 (&S)[16], float dt, int steps, __half* y, size_t yp, int pcols) {
+__device__ __forceinline__ void chunk_plain(unsigned char* smem, ChunkTail* tail, const Lane& t, f2 (&S)[16], float dt, int steps, __half* y, size_t yp, int pcols, int ncols) {
   float* held = reinterpret_cast<float*>(smem + CK_T) + t.half * 32 * CN + t.row;
 #pragma unroll
   for (int p = 0; p < 16; ++p) {
@@ -295,7 +295,7 @@ __device__ __forceinline__ void chunk_plain(unsigned char* smem, ChunkTail* tail
 #pragma unroll
     for (int p = 0; p < 32; ++p) {
       const float x = __half2float(*reinterpret_cast<const __half*>(smem + CK_X + ck_at(i, t.half * 4 + (p >> 3)) + (p & 7) * 2));
-      const float now = a * held[p * CN] + d * x * b;
+      const float now = t.row < ncols ? a * held[p * CN] + d * x * b : 0.f;      // (columns behind the last: an infinity times nothing would reach y)
       held[p * CN] = now;
       v[p] = c * now;
     }
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
         ck_cp_commit();
         ck_cp_wait<0>();
       }
-      chunk_plain<true>(ck_smem, tail, t, S, z.dt, steps, tail->y + t0 * g.yp, g.yp, pcols);
+      chunk_plain<true>(ck_smem, tail, t, S, z.dt, steps, tail->y + t0 * g.yp, g.yp, pcols, g.N);
     } else {
       // (2^60: scores below 2^-47 do not show in y, and the state's share, which takes the same scale, stays finite)
       const Scale sv = ck_scale(v_most), sw = ck_scale(w_most, 60);
@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
     }
     left *= total;
     if (odd || ck_infinite(v_most)) {
-      chunk_plain<false>(ck_smem, tail, t, S, z.dt, CQ, nullptr, 0, pcols);
+      chunk_plain<false>(ck_smem, tail, t, S, z.dt, CQ, nullptr, 0, pcols, g.N);
     } else {
       const Scale sv = ck_scale(v_most);
       store_v(base + CK_T, base + CK_X, t.row, t.half, w * sv.up);

@@ -49,6 +49,8 @@ class Generator:
         model = weights if hasattr(weights, "w16") else None
         if model is not None and model.cfg.param_shapes() != cfg.param_shapes():
             raise ValueError("the model has another configuration")
+        if model is not None and stream is not None and stream is not model.stream:
+            raise ValueError("a model's buffers are used on the model's stream")
         self._own_stream = stream is None and model is None
         self.stream = stream if stream is not None else model.stream if model is not None else Stream()
         self._lib = lib()
@@ -177,8 +179,9 @@ class Generator:
 
     def token(self, tokens):
         """One new token (int32, device) of each of the first len(tokens) sequences; returns their logits (see `prompt`)."""
+        import torch
         n = tokens.numel()
-        if not 1 <= n <= self.sequences or tokens.element_size() != 4 or not tokens.is_cuda or not tokens.is_contiguous():
+        if not 1 <= n <= self.sequences or tokens.dtype != torch.int32 or not tokens.is_cuda or not tokens.is_contiguous():
             raise ValueError("tokens: up to `sequences` contiguous int32 values on the device")
         self._head(self._layers(tokens, n, 0), n)
         return self.logits[:n]

@@ -294,6 +294,35 @@ def test_chunks_with_an_infinity(mp, stream, long, what, value):
         within(got[fine], want[fine], tol[fine], "finite part")
 
 
+@pytest.mark.parametrize("sfx,shape", [("r16", (2, 64, 40, 1)), ("r16", (2, 64, 77, 1)), ("r32", (2, 33, 77, 1)), ("r32", (2, 64, 128, 1)), ("r64", (2, 16, 5, 2)), ("r32", (1, 8, 200, 1))])
+@pytest.mark.parametrize("lens", [[37, 5], [700, 3]])
+@pytest.mark.parametrize("what", ["x", "rate"])
+def test_infinities_beside_padding(mp, stream, sfx, shape, lens, what):
+    """State sizes that fill no tile: an infinite x among positive B and C makes y infinite, not undefined; a head that forgets at once (its decay
+    is exactly zero) keeps the last step only."""
+    r = np.random.default_rng(sum(shape))
+    starts, slots, resume, rows = ref.packed(r, lens, 3)
+    resume[:] = 1
+    s = Scan(r, sfx, rows, 3, *shape, behind=8)
+    s.xbc[:, s.inner:] = np.abs(s.xbc[:, s.inner:]) + NP_OF[sfx](0.125)
+    if what == "x":
+        s.xbc[starts[1] - 2, 1] = np.inf
+    else:
+        s.A_log[0] = np.inf
+    y, states = s.go(mp, stream, slots, resume, starts)
+    with np.errstate(all="ignore"):
+        wy, ysize, ws, ssize, ysteps, ssteps = s.want(starts, slots, resume)
+    H, P, N, G = s.dims
+    y = y[:, :s.inner].reshape(-1, H, P)
+    with np.errstate(all="ignore"):
+        ytol, stol = ref.scan_tolerance(sfx, wy, ysize, ysteps, N, True), ref.scan_tolerance(sfx, ws, ssize, ssteps, N, False)
+    for got, want, tol in ((y[:starts[-1]], wy[:starts[-1]], np.broadcast_to(ytol, wy.shape)[:starts[-1]]), (states[slots], ws[slots], np.broadcast_to(stol, ws.shape)[slots])):
+        got = got.astype(np.float64)
+        assert np.array_equal(np.isinf(got), np.isinf(want)) and not np.isnan(got).any()
+        fine = np.isfinite(want)
+        within(got[fine], want[fine], tol[fine], "finite part")
+
+
 # ---------------------------------------------------------------------------------------------------- selection
 def select(mp, stream, sfx, logits, scores, finished, eos, picks, off=0):
     import torch
