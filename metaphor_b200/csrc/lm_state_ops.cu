@@ -52,6 +52,8 @@ __device__ __forceinline__ StVec<T, V> silu_vec(const typename Acc<T>::type (&v)
 // Convolution over packed prompts.  A thread has V channels and a run of `run` rows, which it walks with the last W - 1 inputs in registers.
 // Rows that reach into the kept state (the first W - 1 of a sequence) belong to the thread that has the sequence's first row, even behind its
 // run's end, and that thread writes the new state too, from inputs that it fetches again: so nobody else reads what it overwrites.
+// Measured (r16, 16 prompts of 8264 rows in all, 1792 channels): 17.5 us, 3.0 TB/s.  The special-function unit, which gives 16 of a value's two
+// results a clock, is busy for 6.6 us of it; the rest is the way to the first inputs (sequence, state, taps) and too few warps to hide it.
 // ---------------------------------------------------------------------------
 constexpr int CS_TX = 32, CS_TY = 4, CS_U = 8;
 
@@ -193,7 +195,8 @@ __global__ void __launch_bounds__(128) conv_token_kernel(const T* x, size_t xp, 
 // ---------------------------------------------------------------------------
 // Scan of one token per sequence:  S = exp(dt A) S + dt x (x) B,  y = S C.  The state ([P][N], accumulator type) is read and written once and
 // is nearly all of the traffic.  L lanes have a row p of it, V values at a time; a warp takes ST_U rows per lane group at a time, `batches` times,
-// so that what a row costs beside its own values (step size, B and C, addresses) is shared.  The ST_U sums of a lane group are added up across
+// so that what a row costs beside its own values (step size, B and C, addresses) is shared.  Measured (r16, 24 heads of 64 x 128): 300 tokens 82 us,
+// 5.8 TB/s of the 6.5 that a copy has; one token 4.4 us, the way to the state and a launch.  The ST_U sums of a lane group are added up across
 // its lanes by halves: in each of three rounds a lane hands on half of its sums and keeps the others.
 // ---------------------------------------------------------------------------
 constexpr int ST_U = 8;
@@ -283,6 +286,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 8 ? 3 : 6) scan_token_kernel
 // States that follow the beams, in place.  The CTA lists the beams that another one follows (each is read once) and the beams that change
 // (each is written once); beams that keep their state cost nothing.  A thread has W bytes of every state of one search, RE_TURNS times: it
 // fetches them into shared memory, the next turn's while this one's are written.  No other thread touches these bytes, so no barrier stands between.
+// Measured (24 layers, 8 searches of 5 beams, rows of 768 KB): 152 us, 5.97 TB/s of the 6.5 that a copy has; with one word a thread and the lists
+// made out by every thread, 185.
 // ---------------------------------------------------------------------------
 constexpr int RE_BEAMS = 64, RE_STAGES = 2;
 

@@ -12,6 +12,9 @@ namespace {
 // instruction in fp32: bound by the fp32 pipe.  A lane leaves its share of y_t in shared memory; the LN shares of a value are added up behind
 // the RT steps, so that no step waits for shuffles.  More lanes to a row make more and smaller CTAs; fewer rows to a lane would too, but then
 // B and C, of which a lane reads as many values as it has columns, would come from shared memory no faster than now for a quarter of the products.
+// Measured (r32, 64 rows and 128 columns a head): one prompt of 4095 steps and 24 heads 206 us, 12 of up to 1200 375 us (half of the fp32 pipe's
+// rate), one of 37 steps 10 us (0.1 us a step: one warp on each scheduler, and a step's reads of shared memory and sums in a row); r64, 4 heads,
+// three of up to 900 steps 61 us.
 // Where the sequences and heads are too few for the GPU, long sequences are cut into ranges: first the states that all but the last ranges add
 // (`STATES`: from zero, without y), then carried from range to range, then the ranges side by side from the states that they receive.
 // ---------------------------------------------------------------------------
