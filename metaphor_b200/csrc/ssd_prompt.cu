@@ -12,9 +12,9 @@ namespace {
 // instruction in fp32: bound by the fp32 pipe.  A lane leaves its share of y_t in shared memory; the LN shares of a value are added up behind
 // the RT steps, so that no step waits for shuffles.  More lanes to a row make more and smaller CTAs; fewer rows to a lane would too, but then
 // B and C, of which a lane reads as many values as it has columns, would come from shared memory no faster than now for a quarter of the products.
-// Measured (r32, 64 rows and 128 columns a head): one prompt of 4095 steps and 24 heads 206 us, 12 of up to 1200 375 us (half of the fp32 pipe's
-// rate), one of 37 steps 10 us (0.1 us a step: one warp on each scheduler, and a step's reads of shared memory and sums in a row); r64, 4 heads,
-// three of up to 900 steps 61 us.
+// Measured (r32, 64 rows and 128 columns a head): one prompt of 4095 steps and 24 heads 203 us, 12 of up to 1200 369 us (half of the fp32 pipe's
+// rate), one of 37 steps 8 us (0.1 us a step: one warp on each scheduler, and a step's reads of shared memory and sums in a row); r64, 4 heads,
+// three of up to 900 steps 51 us (61 with the step sizes made by one of the four warps: the others wait for it).
 // Where the sequences and heads are too few for the GPU, long sequences are cut into ranges: first the states that all but the last ranges add
 // (`STATES`: from zero, without y), then carried from range to range, then the ranges side by side from the states that they receive.
 // ---------------------------------------------------------------------------
@@ -68,7 +68,7 @@ __device__ __forceinline__ void fetch_rows(typename Acc<T>::type* dst, const T* 
 }
 
 template <typename T, int NP, int LN, bool STATES>
-__global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, const Ranges ranges, int splits) {
+__global__ void __launch_bounds__(160, 3) recurrence_kernel(const PromptArgs g, const Ranges ranges, int splits) {
   mp_grid_dependency();
   using Z = RecurrenceSizes<T, NP, LN>;
   using A = typename Z::A;
@@ -77,6 +77,8 @@ __global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, 
   // a tile: B [RT][NP], columns past N zero; C the same; x [RT][PS]; decays [RT]; step sizes [RT]
   A* shares = reinterpret_cast<A*>(rc_smem) + 2 * Z::TILE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // a fifth warp makes the step sizes and decays of the next tile: exponential and logarithm are as long as several steps
+  const bool helper = warp == Z::WARPS;
   const int split = blockIdx.x % splits, idh = blockIdx.x / splits, h = idh % g.H, grp = h / (g.H / g.G);
   const Span sp = span_of(g.q, ranges.steps, idh / g.H);
   if (!sp.any || (STATES && sp.hi >= sp.seq_hi)) return;      // (nothing lies behind it)
@@ -93,7 +95,7 @@ __global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, 
   // a lane's columns are neighbours CV at a time: 16-byte reads of B and C, the lanes of a row next to each other
   A S[PV][NV / CV][CV];
   auto column = [&](int i, int e) { return (i * LN + nl) * CV + e; };
-  const bool received = !STATES && ranges.steps != 0 && sp.lo > sp.seq_lo, any = received || (!STATES && seq_resumes(g.q, sp.s));
+  const bool received = !STATES && ranges.steps != 0 && sp.lo > sp.seq_lo, any = !helper && (received || (!STATES && seq_resumes(g.q, sp.s)));
   const A* from = received ? local : state;
   const bool vectors = g.N % CV == 0 && mp_aligned16(g.states);
 #pragma unroll
@@ -115,20 +117,21 @@ __global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, 
       for (int e = 0; e < CV; ++e) S[p][i][e] = v.v[e];
     }
 
-  // (raw step sizes are asked for a tile earlier: one warp would wait for them, and all others for it)
-  auto raw_at = [&](long long t0) { return tid < RT && t0 + tid < sp.hi ? mp_up(raw[(t0 + tid) * g.rp]) : A(0); };
+  // (raw step sizes are asked for a tile earlier)
+  auto raw_at = [&](long long t0) { return helper && lane < RT && t0 + lane < sp.hi ? mp_up(raw[(t0 + lane) * g.rp]) : A(0); };
   A raw_here = raw_at(sp.lo);
   auto fetch = [&](long long t0) {
     A* tile = reinterpret_cast<A*>(rc_smem) + ((t0 - sp.lo) / RT & 1) * Z::TILE;
     const int steps = sp.hi - t0 < RT ? static_cast<int>(sp.hi - t0) : RT;
-    fetch_rows<T, NP, RT, THREADS>(tile, Bm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
-    if (!STATES) fetch_rows<T, NP, RT, THREADS>(tile + RT * NP, Cm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
-    fetch_rows<T, PS, RT, THREADS>(tile + 2 * RT * NP, x + t0 * g.xp, g.xp, steps, g.P - split * PS, ranges.packs);
-    if (tid < RT) {
-      const A dt = tid < steps ? seq_softplus(raw_here + bias) : A(0);
+    if (!helper) {
+      fetch_rows<T, NP, RT, THREADS>(tile, Bm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
+      if (!STATES) fetch_rows<T, NP, RT, THREADS>(tile + RT * NP, Cm + t0 * g.bcp, g.bcp, steps, g.N, ranges.packs);
+      fetch_rows<T, PS, RT, THREADS>(tile + 2 * RT * NP, x + t0 * g.xp, g.xp, steps, g.P - split * PS, ranges.packs);
+    } else if (lane < RT) {
+      const A dt = lane < steps ? seq_softplus(raw_here + bias) : A(0);
       raw_here = raw_at(t0 + RT);
-      tile[2 * RT * NP + RT * PS + tid] = tid < steps ? seq_exp(dt * rate) : A(1);
-      tile[2 * RT * NP + RT * PS + RT + tid] = dt;
+      tile[2 * RT * NP + RT * PS + lane] = lane < steps ? seq_exp(dt * rate) : A(1);
+      tile[2 * RT * NP + RT * PS + RT + lane] = dt;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -139,55 +142,59 @@ __global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, 
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     if (t0 + RT < sp.hi) fetch(t0 + RT);
+    if (helper) continue;
     const A* sB = reinterpret_cast<const A*>(rc_smem) + ((t0 - sp.lo) / RT & 1) * Z::TILE;
     const A *sC = sB + RT * NP, *sx = sC + RT * NP, *sa = sx + RT * PS, *sdt = sa + RT;
     // UN steps at a time, so that one's operands are read and its sums finished beside another one's products; steps behind the last have a size
     // of zero and change nothing.  (The shares are stored behind all of them: no read of a tile may pass a store.)
     constexpr int UN = NV <= 4 ? 4 : 2;
-    for (int tu = 0; tu < steps; tu += UN) {
-      StVec<A, PV> total[UN];
+    auto work = [&](auto padded) {
+      for (int tu = 0; tu < steps; tu += UN) {
+        StVec<A, PV> total[UN];
 #pragma unroll
-      for (int q = 0; q < UN; ++q) {
-        const int t = tu + q;
-        A a[CV], xd[PV][CV], sum[PV][CV];
-        const A dt = sdt[t], a1 = sa[t];
-        if (STATES) left *= a1;
+        for (int q = 0; q < UN; ++q) {
+          const int t = tu + q;
+          A a[CV], xd[PV][CV], sum[PV][CV];
+          const A dt = sdt[t], a1 = sa[t];
+          if (STATES) left *= a1;
 #pragma unroll
-        for (int e = 0; e < CV; ++e) a[e] = a1;
-#pragma unroll
-        for (int p = 0; p < PV; ++p) {
-          const A v = dt * sx[t * PS + pl + p];
-#pragma unroll
-          for (int e = 0; e < CV; ++e) { xd[p][e] = v; sum[p][e] = A(0); }
-        }
-#pragma unroll
-        for (int i = 0; i < NV / CV; ++i) {
-          const StVec<A, CV> b = *reinterpret_cast<const StVec<A, CV>*>(sB + t * NP + column(i, 0));
-          StVec<A, CV> c;
-          if (!STATES) c = *reinterpret_cast<const StVec<A, CV>*>(sC + t * NP + column(i, 0));
+          for (int e = 0; e < CV; ++e) a[e] = a1;
 #pragma unroll
           for (int p = 0; p < PV; ++p) {
-            mul_vec(S[p][i], a, S[p][i]);
-            fma_vec(S[p][i], xd[p], b.v, S[p][i]);
-            if ((i + 1) * LN * CV > g.N) {      // columns behind the last stay zero: an infinity times nothing would reach y
+            const A v = dt * sx[t * PS + pl + p];
 #pragma unroll
-              for (int e = 0; e < CV; ++e) S[p][i][e] = column(i, e) < g.N ? S[p][i][e] : A(0);
+            for (int e = 0; e < CV; ++e) { xd[p][e] = v; sum[p][e] = A(0); }
+          }
+#pragma unroll
+          for (int i = 0; i < NV / CV; ++i) {
+            const StVec<A, CV> b = *reinterpret_cast<const StVec<A, CV>*>(sB + t * NP + column(i, 0));
+            StVec<A, CV> c;
+            if (!STATES) c = *reinterpret_cast<const StVec<A, CV>*>(sC + t * NP + column(i, 0));
+#pragma unroll
+            for (int p = 0; p < PV; ++p) {
+              mul_vec(S[p][i], a, S[p][i]);
+              fma_vec(S[p][i], xd[p], b.v, S[p][i]);
+              if constexpr (decltype(padded)::value) {      // columns behind the last stay zero: an infinity times nothing would reach y
+#pragma unroll
+                for (int e = 0; e < CV; ++e) S[p][i][e] = column(i, e) < g.N ? S[p][i][e] : A(0);
+              }
+              if (!STATES) fma_vec(sum[p], c.v, S[p][i], sum[p]);
             }
-            if (!STATES) fma_vec(sum[p], c.v, S[p][i], sum[p]);
+          }
+#pragma unroll
+          for (int p = 0; p < PV; ++p) {
+            total[q].v[p] = sum[p][0];
+#pragma unroll
+            for (int e = 1; e < CV; ++e) total[q].v[p] += sum[p][e];
           }
         }
+        if (!STATES) {
 #pragma unroll
-        for (int p = 0; p < PV; ++p) {
-          total[q].v[p] = sum[p][0];
-#pragma unroll
-          for (int e = 1; e < CV; ++e) total[q].v[p] += sum[p][e];
+          for (int q = 0; q < UN; ++q) *reinterpret_cast<StVec<A, PV>*>(shares + ((tu + q) * THREADS + tid) * PV) = total[q];
         }
       }
-      if (!STATES) {
-#pragma unroll
-        for (int q = 0; q < UN; ++q) *reinterpret_cast<StVec<A, PV>*>(shares + ((tu + q) * THREADS + tid) * PV) = total[q];
-      }
-    }
+    };
+    if (g.N < NP) work(std::true_type()); else work(std::false_type());
     if (!STATES) {
       __syncwarp();
       // a lane has one of the warp's ROWS values of every (32 / ROWS)-th step; it begins with another one of the shares than its
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(128, 4) recurrence_kernel(const PromptArgs g, 
     }
   }
   A* to = STATES ? local : state;
-  if (!STATES && sp.hi < sp.seq_hi) return;
+  if (helper || (!STATES && sp.hi < sp.seq_hi)) return;
 #pragma unroll
   for (int p = 0; p < PV; ++p)
 #pragma unroll
@@ -266,9 +273,11 @@ __global__ void __launch_bounds__(256) recurrence_carry_kernel(const PromptArgs 
 
 // How a call is cut up.  The host knows how many sequences and rows there are, not how long each is.
 struct Cut { int lanes, splits, steps; size_t ids; };      // lanes of a row; CTAs of a head; steps of a range (0: whole sequences); ranges or sequences
-// `least`, `most`: lanes of a row; `held`: rows p of a lane.  Ranges of 64 steps or more where a sequence may be long and there are not twice as many
-// CTAs as the GPU holds (four for each of 148 SMs) all the same: a range's state is made twice.  Rows get more lanes where a head is small, or
-// where there are too few CTAs.
+// `least`, `most`: lanes of a row; `held`: rows p of a lane.  Ranges of 32 steps or more where a sequence may be longer than 320 steps and there
+// are not eight CTAs for each of 148 SMs all the same (three fit at a time): a range's state is made twice.  Measured, r32, whole and in ranges: one
+// sequence of 256 steps and 24 heads 28 and 46 us, of 512 steps 52 and 44, with 4 heads 51 and 22; and that with
+// ranges of 64 at least 25.  Rows get more lanes where a head is small, or where there are fewer than two CTAs for an SM (12 sequences of up to 300
+// steps: 95 us, with one CTA for an SM 143, with four 105).
 Cut recurrence_cut(size_t nseq, size_t rows, size_t heads, size_t headdim, int held, int least, int most) {
   Cut c{least, 0, 0, nseq};
   auto rows_of = [&] { return static_cast<size_t>(held) * (128 / c.lanes); };
@@ -278,7 +287,7 @@ Cut recurrence_cut(size_t nseq, size_t rows, size_t heads, size_t headdim, int h
   if (nseq * units < 8 * 148 && longest > 320) {
     const size_t want = 8 * 148 / units + 1;
     size_t range = ((rows + want - 1) / want + 15) / 16 * 16;
-    if (range < 64) range = 64;
+    if (range < 32) range = 32;
     if (range < rows) { c.steps = static_cast<int>(range); c.ids = rows / range + nseq; }
   }
   while (c.lanes < most && c.ids * heads * splits() < 2 * 148) c.lanes <<= 1;
@@ -294,7 +303,7 @@ void recurrence_run(const PromptArgs& g, const Ranges& r, const Cut& c, StreamCo
   if (ctas > 0x7fffffffull) MP_FATAL("ssd_scan_prompt: too many sequences and heads for one launch");
   auto go = [&](auto kernel) {
     if (Z::BYTES > 48 * 1024) MP_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Z::BYTES)));
-    MpLaunch(static_cast<unsigned>(ctas), Z::THREADS, Z::BYTES, mp_stream(ctx))(kernel, g, r, c.splits);
+    MpLaunch(static_cast<unsigned>(ctas), Z::THREADS + 32, Z::BYTES, mp_stream(ctx))(kernel, g, r, c.splits);
     MP_LAUNCH_CHECK();
   };
   if (r.steps != 0) {
