@@ -275,8 +275,7 @@ __global__ void __launch_bounds__(256) recurrence_carry_kernel(const PromptArgs 
 struct Cut { int lanes, splits, steps; size_t ids; };      // lanes of a row; CTAs of a head; steps of a range (0: whole sequences); ranges or sequences
 // `least`, `most`: lanes of a row; `held`: rows p of a lane.  Ranges of 32 steps or more where a sequence may be longer than 320 steps and there
 // are not eight CTAs for each of 148 SMs all the same (three fit at a time): a range's state is made twice.  Measured, r32, whole and in ranges: one
-// sequence of 256 steps and 24 heads 28 and 46 us, of 512 steps 52 and 44, with 4 heads 51 and 22; and that with
-// ranges of 64 at least 25.  Rows get more lanes where a head is small, or where there are fewer than two CTAs for an SM (12 sequences of up to 300
+// sequence of 256 steps and 24 heads 28 and 46 us, of 512 steps 52 and 44, with 4 heads 51 and 22 (25 with ranges of 64 steps at least).  Rows get more lanes where a head is small, or where there are fewer than two CTAs for an SM (12 sequences of up to 300
 // steps: 95 us, with one CTA for an SM 143, with four 105).
 Cut recurrence_cut(size_t nseq, size_t rows, size_t heads, size_t headdim, int held, int least, int most) {
   Cut c{least, 0, 0, nseq};

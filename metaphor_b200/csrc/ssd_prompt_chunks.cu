@@ -16,7 +16,7 @@
 // Measured (r16, 64 rows and 128 columns a head, one group): 16 prompts of up to 1023 steps and 24 heads 72 us, where the bytes would take 10.4 and
 // 126 MMAs of 128 x 64 x 16 a chunk 21 % of the time.  A chunk takes a CTA about 8 us beside another one, eight of them in a row for the longest
 // prompt: the scaling between the products (weights, two terms per value, sums) is what it waits for, a third of it the way through barriers.
-// One prompt of 8191 steps and 32 heads 112 us (states 25, carry 8, walk 75), one of 37 steps and 24 heads 8.7 us.
+// One prompt of 8191 steps and 32 heads 112 us (states 32, carry 5, walk 75), one of 37 steps and 24 heads 8.7 us.
 //
 // A chunk with an infinity or a NaN among its values does not go through the products, where a zero weight would spread it: it is taken step by
 // step (chunk_plain).
