@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(160, 3) recurrence_kernel(const PromptArgs g, 
   // a lane's columns are neighbours CV at a time: 16-byte reads of B and C, the lanes of a row next to each other
   A S[PV][NV / CV][CV];
   auto column = [&](int i, int e) { return (i * LN + nl) * CV + e; };
-  const bool received = !STATES && ranges.steps != 0 && sp.lo > sp.seq_lo, any = !helper && (received || (!STATES && seq_resumes(g.q, sp.s)));
+  // (the first of several ranges too has what it receives in `local`: the last one may be writing the sequence's state by now)
+  const bool received = !STATES && ranges.steps != 0 && sp.seq_hi - sp.seq_lo > ranges.steps, any = !helper && (received || (!STATES && seq_resumes(g.q, sp.s)));
   const A* from = received ? local : state;
   const bool vectors = g.N % CV == 0 && mp_aligned16(g.states);
 #pragma unroll
@@ -234,7 +235,8 @@ __global__ void __launch_bounds__(160, 3) recurrence_kernel(const PromptArgs g, 
   if (STATES && split == 0 && tid == 0) static_cast<A*>(ranges.decay)[idh] = left;
 }
 
-// From range to range: what each adds is replaced by what it receives.  A thread has one value of a state, four ranges' on their way.
+// From range to range: what each adds is replaced by what it receives, the first one by the kept state.  A thread has one value of a state, four
+// ranges' on their way.
 template <typename A>
 __global__ void __launch_bounds__(256) recurrence_carry_kernel(const PromptArgs g, const Ranges ranges, int parts) {
   mp_grid_dependency();
@@ -251,6 +253,7 @@ __global__ void __launch_bounds__(256) recurrence_carry_kernel(const PromptArgs 
   const size_t next = static_cast<size_t>(g.H) * size;
   constexpr int U = 4;
   A ahead = at[0];      // (place j + 1 is read before it is written: what its range adds goes to the one behind)
+  at[0] = v;
   for (long long j = 0; j + 1 < n; j += U) {
     A add[U + 1], left[U];
     add[0] = ahead;

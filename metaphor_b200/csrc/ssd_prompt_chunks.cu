@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
     const float* from = state;
     long long pitch = g.N;
     bool any = true;
-    if (a.range != 0 && sp.lo > sp.seq_lo) {
+    if (a.range != 0 && sp.seq_hi - sp.seq_lo > a.range) {      // (the first range too: the last one may be writing the sequence's state by now)
       from = a.local + (static_cast<size_t>(id) * units + unit) * CP * CN;
       pitch = CN;
     } else {
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
   if (t.warp == 0) tmem_dealloc(tmem, CP);
 }
 
-// From range to range: what each adds is replaced by what it receives.  A thread has four neighbouring values of a state.
+// From range to range: what each adds is replaced by what it receives, the first one by the kept state.  A thread has four neighbouring values of a state.
 constexpr int CR_PARTS = CP * CN / 4 / 256;
 __global__ void __launch_bounds__(256) chunk_carry_kernel(const ChunkArgs a) {
   mp_grid_dependency();
@@ -802,6 +802,7 @@ __global__ void __launch_bounds__(256) chunk_carry_kernel(const ChunkArgs a) {
   // eight ranges on their way at a time: one after the other is a trip to the L2 each (one prompt of 8191 steps: 114.6 -> 112.1 us)
   constexpr int U = 8;
   float4 ahead = *place(0);      // (place j + 1 is read before it is written: what its range adds goes to the one behind)
+  *place(0) = v;
   for (long long j = 0; j + 1 < ranges; j += U) {
     float4 add[U + 1];
     float left[U];

@@ -323,6 +323,23 @@ def test_infinities_beside_padding(mp, stream, sfx, shape, lens, what):
         within(got[fine], want[fine], tol[fine], "finite part")
 
 
+@pytest.mark.parametrize("sfx", TYPES)
+def test_ranges_begin_with_the_kept_state(mp, stream, sfx):
+    """Long prompts that go on from a state, the last range of a single step: the first range begins with the state that was kept, not with the one
+    that the last range leaves.  The same bits every time."""
+    r = np.random.default_rng(50)
+    lens = [1024 * 2 + 1, 1537]
+    starts, slots, resume, rows = ref.packed(r, lens, 3)
+    resume[:] = 1
+    s = Scan(r, sfx, rows, 3, 2, 64, 128, 1, behind=8)
+    s.states *= 30
+    first = s.go(mp, stream, slots, resume, starts)
+    s.check(first, starts, slots, resume)
+    for _ in range(4):
+        again = s.go(mp, stream, slots, resume, starts)
+        assert np.array_equal(again[0], first[0]) and np.array_equal(again[1], first[1])
+
+
 # ---------------------------------------------------------------------------------------------------- selection
 def select(mp, stream, sfx, logits, scores, finished, eos, picks, off=0):
     import torch
