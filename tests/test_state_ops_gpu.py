@@ -559,3 +559,65 @@ def test_two_streams_at_once(mp, stream):
         st.close()
     for s, w, (_, states) in zip((a, b), want, alone):
         assert np.array_equal(host(s.d["y0"]), w) and np.array_equal(host(s.d["states"]), states)
+
+
+@pytest.mark.parametrize("sfx", ["r16", "r32"])
+def test_prompts_captured_and_replayed(mp, stream, sfx):
+    """Convolution and scan of prompts (in ranges) in a graph: the bits of the same launches one by one, as often as it is replayed."""
+    import torch
+    r = np.random.default_rng(17)
+    lens, heads, width = [700, 0, 33], 2, 4
+    starts, slots, resume, rows = ref.packed(r, lens, 4)
+    resume[:] = 1
+    channels, t = heads * 64 + 256, torch_dtype(sfx)
+    size = np.dtype(NP_OF[sfx]).itemsize
+    base = dict(zx=ref.storage(r, (rows, channels + 8), sfx), w=ref.storage(r, (channels, width), sfx, 0.5), conv=ref.storage(r, (4, width - 1, channels), sfx),
+                ssm=r.standard_normal((4, heads, 64, 128)).astype(np.float32), dt_bias=np.full(heads, -3, np.float32), A_log=np.zeros(heads, np.float32),
+                starts=starts, slots=slots, resume=resume)
+    lib = mp.lib()
+
+    def fresh():
+        d = {k: dev(v) for k, v in base.items()}
+        d.update(xbc=torch.zeros(rows, channels, dtype=t, device="cuda"), y=torch.zeros(rows, heads * 64, dtype=t, device="cuda"),
+                 scratch=torch.zeros(lib.mpSsdScanPromptScratchBytes(TYPES.index(sfx), 3, rows, heads, 64, 128, 1), dtype=torch.uint8, device="cuda"))
+        torch.cuda.synchronize()
+        return d
+
+    def issue(d, st):
+        mp.launch("causal_conv1d_silu_prompt", t, d["zx"], channels + 8, d["w"], None, d["conv"], d["slots"], d["resume"], d["starts"], d["xbc"], channels, 3, rows, 4,
+                  channels, width, st)
+        x = d["xbc"].data_ptr()
+        mp.launch("ssd_scan_prompt", t, x, channels, d["zx"].data_ptr() + channels * size, channels + 8, d["dt_bias"], d["A_log"], x + heads * 64 * size,
+                  x + (heads * 64 + 128) * size, channels, d["ssm"], d["slots"], d["resume"], d["starts"], d["y"], heads * 64, d["scratch"], 3, rows, 4, heads, 64, 128, 1, st)
+
+    plain, graphed = fresh(), fresh()
+    with mp.Stream() as st:
+        for _ in range(3):
+            issue(plain, st)
+        st.sync()
+        lib.mpGraphBeginCapture(st.ctx)
+        issue(graphed, st)
+        graph = lib.mpGraphEndCapture(st.ctx)
+        for _ in range(3):
+            lib.mpGraphLaunch(C.c_void_p(graph), st.ctx)
+        st.sync()
+        assert st.status() == 0
+        lib.mpGraphDestroy(C.c_void_p(graph))
+    for k in ("conv", "ssm", "xbc", "y"):
+        assert torch.equal(plain[k], graphed[k]), k
+
+
+@pytest.mark.parametrize("sfx", TYPES)
+def test_select_any_offset_gives_the_same(mp, stream, sfx):
+    """Rows on the 16-byte boundary and off it by every possible offset: the same bits, and equal rows tie whatever their addresses."""
+    r = np.random.default_rng(23)
+    vocab, beams, picks = 4003, 4, 8
+    one = ref.storage(r, (1, 1, vocab), sfx, 2.0)
+    logits = np.repeat(one, beams, axis=1)
+    scores = np.zeros((1, beams), ref.ACC[sfx])
+    want = None
+    for off in range(16 // np.dtype(NP_OF[sfx]).itemsize + 1):
+        got = select(mp, stream, sfx, logits, scores, None, vocab, picks, off)
+        assert np.array_equal(got[1][0], np.arange(picks) % beams) and np.array_equal(got[2][0], np.repeat(got[2][0][::beams], beams)), off
+        want = got if want is None else want
+        assert all(np.array_equal(a, b) for a, b in zip(got[:3], want[:3])), off
