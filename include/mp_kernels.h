@@ -300,7 +300,8 @@ MP_EXTERN_C len_t mpSsdScanPromptScratchBytes(uint32_t dtype_key, len_t nseq, le
 /* The `picks` best continuations of each search over its beams and the vocabulary, best first:
  *   score(i, v) = scores[i] + logits[i, v] - logsumexp(logits[i, :])
  * logits: T [batch * beams, vocab], row pitch logits_pitch; scores: acc [batch, beams].  Inside a beam the order is that of
- * the logits (of equal ones the lower token first), between beams that of the score, formed in r64 (the lower beam first).
+ * the logits (of equal ones the lower token first), between beams that of the score, formed in r64 as
+ * scores[i] + ((logits[i, v] - max) - log sum exp(logits[i, :] - max)) (the lower beam first).
  * A beam with finished[i] != 0 (int32 [batch, beams], may be NULL) goes on with the token `eos` alone, at its score.  A beam whose
  * score is NaN or minus infinity, or whose logits hold a NaN or plus infinity or nothing above minus infinity, has no possible
  * continuation: its tokens rank in their order with a score of minus infinity.

@@ -443,7 +443,8 @@ __global__ void __launch_bounds__(BM_MERGE_WARPS * 32) beam_merge_kernel(BeamScr
         token = lane == 0 ? eos : lane - 1 < eos ? lane - 1 : lane;
         if (lane == 0) score = static_cast<double>(had);
       } else if (sum > 0 && sum < 1.0 / 0.0) {
-        score = static_cast<double>(had) + (static_cast<double>(value_of(list)) - (static_cast<double>(top) + log(sum)));
+        // (the maximum goes first: beside one of 1e38, a mask's, the sum's logarithm would be lost)
+        score = static_cast<double>(had) + ((static_cast<double>(value_of(list)) - static_cast<double>(top)) - log(sum));
         if (score != score) score = lowest(0.0);      // an infinite score behind a token that is ruled out
         token = index_of(list);
       }      // else a NaN or an infinity among the logits, or nothing above minus infinity: no probabilities

@@ -21,7 +21,17 @@ def _has_gpu() -> bool:
         return False
 
 
+# Tests that hold a wrong value, and the proof: they run on, and are expected to fail.
+_LOST_LOG = ("the oracle forms row - (top + log(sum)): beside a row of the lowest r32 or r64 value the sum's logarithm is lost, so that each of 500 equal "
+             "tokens gets probability 1 (score -30) instead of 1/500 (-30 - ln 500 = -36.2); test_select_masked_and_impossible_rows has the right ones")
+WRONG_VALUES = {f"test_state_ops_gpu.py::test_select_masked_and_impossible[{sfx}]": _LOST_LOG for sfx in ("r32", "r64")}
+
+
 def pytest_collection_modifyitems(config, items):
+    for item in items:
+        reason = next((why for name, why in WRONG_VALUES.items() if item.nodeid.endswith(name)), None)
+        if reason is not None:
+            item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
     if _has_gpu():
         return
     skip = pytest.mark.skip(reason="no CUDA device in this container")
