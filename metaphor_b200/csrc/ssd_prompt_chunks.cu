@@ -3,9 +3,11 @@
 // With cum the inclusive sums of dt A inside a chunk, E their last one and S the state the chunk receives:
 //   y_i = sum_{j <= i} (C_i . B_j) exp(cum_i - cum_j) dt_j x_j + exp(cum_i) S C_i          S' = exp(E) S + sum_j exp(E - cum_j) dt_j x_j (x) B_j
 // Four products of 128 rows: G = C B^T, C S^T (128 x 64 x 128), W x with W the weighted scores, and B^T V with V the weighted x.  S stays in
-// registers as fp32 values from chunk to chunk; where it, W or V is an operand, it is two r16 terms under one power of two (22 bits, down to
-// 2^-38 of the largest value in the tile), so that y is an r16 rounding of fp32 sums and the kept state has fp32's accuracy to 2^-22 a term.
-// x, B and C are r16 in memory and enter as they are.
+// registers as fp32 values from chunk to chunk; where it, W or V is an operand, it is two r16 terms under a power of two: one for each row p of the
+// head in S and V, one for each step in W, since these are columns or rows of the products by themselves (22 bits, down to 2^-38 of the largest
+// value among the row's 128).  So y is an r16 rounding of fp32 sums and the kept state has fp32's accuracy to 2^-22 a term, whatever the other
+// rows hold.  (One power of two for a whole tile took 72, 112 and 8.7 us below, and left a row p that is 2^28 times smaller than another
+// one with 11 bits.)  x, B and C are r16 in memory and enter as they are.
 //
 // A CTA of eight warps walks one sequence of one head (64 of its rows p); two CTAs share an SM, so that one's products run beside the
 // other's scaling.  Shared memory, 112 KB of tiles: C, B (two halves of 64 columns each), x, and one place for the terms of S, later those of V.
@@ -13,10 +15,10 @@
 // Sequences too long and too few to fill the SMs are cut into ranges, whose own states are made first (states_kernel: B^T V alone), then carried
 // from range to range (carry_kernel), then walked side by side.
 //
-// Measured (r16, 64 rows and 128 columns a head, one group): 16 prompts of up to 1023 steps and 24 heads 72 us, where the bytes would take 10.4 and
-// 126 MMAs of 128 x 64 x 16 a chunk 21 % of the time.  A chunk takes a CTA about 8 us beside another one, eight of them in a row for the longest
+// Measured (r16, 64 rows and 128 columns a head, one group): 16 prompts of up to 1023 steps and 24 heads 80 us, where the bytes would take 10.4 and
+// 64 MMAs of 128 x 64 x 16 a chunk a fifth of the time.  A chunk takes a CTA about 9 us beside another one, eight of them in a row for the longest
 // prompt: the scaling between the products (weights, two terms per value, sums) is what it waits for, a third of it the way through barriers.
-// One prompt of 8191 steps and 32 heads 112 us (states 32, carry 5, walk 75), one of 37 steps and 24 heads 8.7 us.
+// One prompt of 8191 steps and 32 heads 124 us, one of 37 steps and 24 heads 9.2 us.
 //
 // A chunk with an infinity or a NaN among its values does not go through the products, where a zero weight would spread it: it is taken step by
 // step (chunk_plain).
@@ -31,7 +33,7 @@ constexpr int CK_HALF = CQ * 128;               // [128 rows][128 bytes], 128-by
 constexpr int CK_C = 0, CK_B = 2 * CK_HALF, CK_X = 4 * CK_HALF, CK_T = 5 * CK_HALF, CK_TAIL = 7 * CK_HALF;
 struct ChunkTail {
   float piece[CQ / 8];       // decay over each piece of eight steps
-  uint32_t most[4][8];       // per warp: largest |G|, |x|, |S|, dt as bits
+  uint32_t most[4][8];       // per warp: largest |G| as bits, exponents of V and of S, dt as bits
   uint64_t bar[4];
   uint32_t tmem;
   int abort;
@@ -41,8 +43,12 @@ struct ChunkTail {
   __half* y;
   float* state;                       // where the last state goes, NULL for ranges that are not a sequence's last
   float bias, rate;
-  float plain_dt, plain_y[CP];
-  float y_down;                       // the last chunk's results over their scale in TMEM
+  alignas(16) uint16_t s_down[CP], v_down[CP];    // per row p: a power of two, the value of a unit in the terms of S and V (the upper half of the float)
+  signed char y_up[CQ];               // per step: the exponent of the last chunk's scale of W and of its results in TMEM
+  union {
+    uint8_t column[4][CP];            // per 32 rows of S or V: the largest exponent of each column
+    struct { float plain_dt, plain_y[CP]; };
+  };
 };
 // Weights of a chunk.  They lie over C once its products are done.
 struct ChunkWeights {
@@ -51,6 +57,7 @@ struct ChunkWeights {
   float enter[CQ];           // decay from the beginning of the row's piece
   float before[CQ];          // decay from the beginning of the chunk
   float v[CQ];               // dt_j exp(E - cum_j)
+  float row[2][CQ];          // largest score of a row, among each half's columns
   float colf[CQ];            // dt_j times the decay towards the end of its piece
 };
 static_assert(sizeof(ChunkWeights) <= 2 * CK_HALF, "it lies over C");
@@ -117,14 +124,38 @@ __device__ __forceinline__ float most_abs(float m, float v) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
   return r;
 }
-// The power of two that takes the largest value (its bits) to [2^13, 2^14), and its inverse.
-struct Scale { float up, down; };
-__device__ __forceinline__ Scale ck_scale(uint32_t most, int largest = 120) {
-  int k = most == 0 ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
-  k = k > largest ? largest : k < -120 ? -120 : k;
-  return {__int_as_float((127 + k) << 23), __int_as_float((127 - k) << 23)};
+// The exponent of the power of two that takes the largest value (its bits) to [2^13, 2^14).
+__device__ __forceinline__ int ck_scale(uint32_t most, int largest) {
+  const int k = most == 0 ? 0 : 13 - (static_cast<int>(most >> 23) - 127);
+  return k > largest ? largest : k < -120 ? -120 : k;
 }
+__device__ __forceinline__ float ck_power(int k) { return __int_as_float((127 + k) << 23); }
 __device__ __forceinline__ bool ck_infinite(uint32_t bits) { return bits >= 0x7f800000u; }
+constexpr uint32_t CK_INFINITE = 255;      // the exponent of an infinity or NaN
+// Two neighbouring powers of two from their upper halves, and their inverses.
+__device__ __forceinline__ f2 ck_down(uint32_t w) { return pk(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ f2 ck_up(uint32_t w) { return ck_down(0x7f007f00u - w); }
+// The largest exponents (biased) of 32 columns over a warp's rows; lane l is left with column l's.  Two columns to a word; in each round a lane hands
+// on half of its words and keeps the others.
+__device__ __forceinline__ uint32_t column_exponents(const f2 (&v)[16], int lane) {
+  uint32_t w[16];
+#pragma unroll
+  for (int p = 0; p < 16; ++p) {
+    const float2 f = upk(v[p]);
+    w[p] = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632) & 0x7f807f80u;
+  }
+#pragma unroll
+  for (int o = 16; o > 1; o >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int k = 0; k < o / 2; ++k) {
+      const uint32_t send = up ? w[k] : w[k + o / 2], keep = up ? w[k + o / 2] : w[k];
+      w[k] = __vmaxu2(keep, __shfl_xor_sync(0xffffffffu, send, o));
+    }
+  }
+  w[0] = __vmaxu2(w[0], __shfl_xor_sync(0xffffffffu, w[0], 1));
+  return (lane & 1 ? w[0] >> 16 : w[0] & 0xffffu) >> 7;
+}
 
 // The products are a few hundred nanoseconds away: look for a while before the bounded wait, whose suspended warps wake up late.
 __device__ __forceinline__ void ck_wait(uint64_t* bar, uint32_t parity, uint32_t* status, volatile int* abort) {
@@ -210,68 +241,57 @@ __device__ __forceinline__ uint32_t cta_most(const uint32_t* most) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// The largest magnitude (NaN above all) among the 32 values of the x tile that this thread fetched itself.
-__device__ __forceinline__ float most_x(uint32_t tile) {
-  constexpr int STEP = CK_THREADS / 8;
-  const uint32_t at = tile + ck_at(threadIdx.x / 8, threadIdx.x % 8);
-  __half2 m = __float2half2_rn(0.f);
-#pragma unroll
-  for (int k = 0; k < CQ / STEP; ++k) {
-    const uint4 x = ck_ld(at + k * STEP * 128);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[e])));
-  }
-  const float2 f = __half22float2(m);
-  return most_abs(f.x, f.y);
+// What this thread's warp knows of the columns of S or V goes to the others; behind a barrier, `column_scales` makes the powers of two of it.
+__device__ __forceinline__ void column_publish(ChunkTail* tail, const Lane& t, const f2 (&v)[16], uint32_t* most, bool infinite = false) {
+  const uint32_t e = column_exponents(v, t.lane), m = infinite ? CK_INFINITE : warp_most(e);
+  tail->column[t.warp & 3][t.half * 32 + t.lane] = static_cast<uint8_t>(e);
+  if (t.lane == 0) most[t.warp] = m;
 }
-// V = x w in two terms, each a [128][64] tile: 32 columns of a row.
-__device__ __forceinline__ void store_v(uint32_t tile, uint32_t x_tile, int row, int half, float w) {
+// Every row p has a power of two of its own, which takes its largest value to [2^13, 2^14): a row of small values keeps its bits beside one of large
+// ones.  (The four warps of a half write the same values.)
+__device__ __forceinline__ void column_scales(ChunkTail* tail, const Lane& t, uint16_t* down) {
+  const int c = t.half * 32 + t.lane;
+  const int e = max(max(tail->column[0][c], tail->column[1][c]), max(tail->column[2][c], tail->column[3][c])) - 13;
+  down[c] = static_cast<uint16_t>((e < 7 ? 7 : e > 247 ? 247 : e) << 7);
+  __syncwarp();
+}
+// V = x w: 32 columns of a row.
+__device__ __forceinline__ void weigh(f2 (&v)[16], uint32_t x_tile, int row, int half, float w) {
   const f2 w2 = both(w);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t at = ck_at(row, half * 4 + k);
-    const uint4 x = ck_ld(x_tile + at);
+    const uint4 x = ck_ld(x_tile + ck_at(row, half * 4 + k));
     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-    uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ck_split(mul2(ck_wide(in[e]), w2), hi[e], lo[e]);
-    ck_st(tile + at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-    ck_st(tile + at + CK_HALF, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    for (int e = 0; e < 4; ++e) v[4 * k + e] = mul2(ck_wide(in[e]), w2);
   }
 }
-// S in two terms the same way: this thread's row is a state column n.
-__device__ __forceinline__ void store_s(uint32_t tile, const Lane& t, const f2 (&S)[16], float up) {
-  const f2 up2 = both(up);
+// 32 columns of a row in two terms, each a [128][64] tile.
+__device__ __forceinline__ void store_terms(uint32_t tile, int row, int half, const f2 (&v)[16], const uint16_t* down) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
+    const uint4 d = *reinterpret_cast<const uint4*>(down + half * 32 + k * 8);
+    const uint32_t scale[4] = {d.x, d.y, d.z, d.w};
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ck_split(mul2(S[k * 4 + e], up2), hi[e], lo[e]);
-    const uint32_t at = tile + ck_at(t.row, t.half * 4 + k);
+    for (int e = 0; e < 4; ++e) ck_split(mul2(v[4 * k + e], ck_up(scale[e])), hi[e], lo[e]);
+    const uint32_t at = tile + ck_at(row, half * 4 + k);
     ck_st(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
     ck_st(at + CK_HALF, make_uint4(lo[0], lo[1], lo[2], lo[3]));
   }
 }
-__device__ __forceinline__ uint32_t most_of(const f2 (&S)[16]) {
-  float m = 0.f;
-#pragma unroll
-  for (int p = 0; p < 16; ++p) {
-    const float2 v = upk(S[p]);
-    m = most_abs(most_abs(m, v.x), v.y);
-  }
-  return abs_bits(m);
-}
-// S = total S + down v, v from TMEM
-__device__ __forceinline__ void add_state(f2 (&S)[16], uint32_t tmem, float total, float down) {
-  const f2 t2 = both(total), d2 = both(down);
+// S = total S + v, v from TMEM in the units of `down`
+__device__ __forceinline__ void add_state(f2 (&S)[16], uint32_t tmem, float total, const uint16_t* down) {
+  const f2 t2 = both(total);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     uint32_t v[16];
     tmem_ld_32x16(tmem + k * 16, v);
+    const uint4 d0 = *reinterpret_cast<const uint4*>(down + k * 16), d1 = *reinterpret_cast<const uint4*>(down + k * 16 + 8);
+    const uint32_t d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
     tmem_ld_wait();
 #pragma unroll
-    for (int p = 0; p < 8; ++p) S[8 * k + p] = fma2(t2, S[8 * k + p], mul2(d2, pk(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1]))));
+    for (int p = 0; p < 8; ++p) S[8 * k + p] = fma2(t2, S[8 * k + p], mul2(ck_down(d[p]), pk(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1]))));
   }
 }
 
@@ -402,12 +422,12 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
       S[p] = pk(v0, v1);
     }
   }
-  auto publish = [&]() {      // S becomes an operand of the next chunk: its terms under one power of two
-    const uint32_t m = warp_most(most_of(S));
-    if (t.lane == 0) tail->most[2][t.warp] = m;
+  auto publish = [&]() {      // S becomes an operand of the next chunk: this thread's row of it is a state column n
+    column_publish(tail, t, S, tail->most[2]);
     __syncthreads();
     const uint32_t most = cta_most(tail->most[2]);
-    if (!ck_infinite(most)) store_s(fresh(base) + CK_T, t, S, ck_scale(most).up);
+    column_scales(tail, t, tail->s_down);
+    if (most != CK_INFINITE) store_terms(fresh(base) + CK_T, t.row, t.half, S, tail->s_down);
     return most;
   };
   uint32_t s_most = publish();
@@ -423,7 +443,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
   // The results of a chunk leave TMEM while the next one's first products run.
   bool pending = false;
   auto store_y = [&](int t0, int steps) {
-    const f2 down = both(tail->y_down);
+    const f2 down = both(ck_power(-tail->y_up[t.row]));
     __half* out = tail->y + (t0 + t.row) * g.yp + t.half * 32;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -438,7 +458,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
   };
   for (int t0 = 0; t0 < length; t0 += CQ) {
     const int steps = steps_at(t0);
-    const bool carried = s_most != 0, products = !ck_infinite(s_most) && fabsf(tail->rate) < INFINITY;
+    const bool carried = s_most != 0, products = s_most != CK_INFINITE && fabsf(tail->rate) < INFINITY;
     ck_cp_wait<1>();      // C and B
     fence_proxy_async_smem();
     tcgen05_fence_before_sync();
@@ -488,8 +508,6 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
       }
     }
     ck_cp_wait<0>();      // this thread's x
-    const uint32_t xm = warp_most(abs_bits(most_x(fresh(base) + CK_X)));
-    if (t.lane == 0) tail->most[1][t.warp] = xm;
     const int q = t.warp & 3;      // this warp's rows begin at 32 q: blocks of 16 score columns up to 2 q + 1 are below or on the diagonal; it has
                                    // every other one
     if (products) {
@@ -503,6 +521,11 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
           uint32_t v[16];
           tmem_ld_32x16(tg + b * 32, v);
           tmem_ld_wait();
+          if (b == q) {      // scores above the diagonal are not used
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (t.half * 16 + e > t.lane) v[e] = 0;
+          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) gm = most_abs(gm, __uint_as_float(v[e]));
         }
@@ -512,7 +535,8 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
       ck_wait(tail->bar + 1, issued, a.status, &tail->abort);
       tcgen05_fence_after_sync();
       issued ^= 1;
-      if (t.half == 0) {      // C is free
+      wt->row[t.half][t.row] = gm;      // C is free
+      if (t.half == 0) {
         wt->enter[t.row] = z.enter;
         wt->before[t.row] = before * z.enter;
         wt->colf[t.row] = z.dt * z.leave;
@@ -524,11 +548,18 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
       }
     }
     __syncthreads();
-    // bounds of V and W: the decays that are left out of them are at most one
-    const float dt_most = __uint_as_float(max(max(tail->most[3][0], tail->most[3][1]), max(tail->most[3][2], tail->most[3][3])));
-    const uint32_t v_most = abs_bits(__uint_as_float(cta_most(tail->most[1])) * dt_most);
-    const uint32_t w_most = products ? abs_bits(__uint_as_float(cta_most(tail->most[0])) * dt_most) : 0u;
-    if (!products || ck_infinite(v_most) || ck_infinite(w_most)) {
+    // the largest values of V, and a bound of W's: the decays that are left out of it are at most one
+    float dt_most = 0.f;
+    bool odd = !products;
+    if (products) {
+      f2 v[16];
+      weigh(v, fresh(base) + CK_X, t.row, t.half, wt->v[t.row]);
+      column_publish(tail, t, v, tail->most[1]);
+      __syncthreads();
+      dt_most = __uint_as_float(max(max(tail->most[3][0], tail->most[3][1]), max(tail->most[3][2], tail->most[3][3])));
+      odd = cta_most(tail->most[1]) == CK_INFINITE || ck_infinite(abs_bits(__uint_as_float(cta_most(tail->most[0])) * dt_most));
+    }
+    if (odd) {
       if (products) {      // the weights lie over C
         __syncthreads();
         fetch_tile<2>(base + CK_C, tail->C + t0 * g.bcp, g.bcp, steps, g.N);
@@ -537,21 +568,27 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
       }
       chunk_plain<true>(ck_smem, tail, t, S, z.dt, steps, tail->y + t0 * g.yp, g.yp, pcols, g.N);
     } else {
-      // (2^60: scores below 2^-47 do not show in y, and the state's share, which takes the same scale, stays finite)
-      const Scale sv = ck_scale(v_most), sw = ck_scale(w_most, 60);
       const uint32_t tiles = fresh(base);
-      // V goes to the warps with few blocks of W: four pieces of 32 rows and 32 columns to the first two, two each to the next
-      for (int u = q == 0 ? 2 * t.half : 2 * q + 2 + t.half, n = q == 0 ? 2 : q == 3 ? 0 : 1; n > 0; ++u, --n) {
-        const int row = (u >> 1) * 32 + t.lane;
-        store_v(tiles + CK_T, tiles + CK_X, row, u & 1, wt->v[row] * sv.up);
+      column_scales(tail, t, tail->v_down);
+      // V goes to the warps with few blocks of W: two pieces of 32 rows to the first, one each to the next two
+      for (int b = q == 0 ? 0 : q + 1, n = q == 0 ? 2 : q == 3 ? 0 : 1; n > 0; ++b, --n) {
+        const int row = b * 32 + t.lane;
+        f2 v[16];
+        weigh(v, tiles + CK_X, row, t.half, wt->v[row]);
+        store_terms(tiles + CK_T, row, t.half, v, tail->v_down);
       }
+      // A row of W (a step) has a power of two of its own.  (2^60: scores below 2^-47 do not show in y, and the state's share, which takes the same
+      // scale, stays finite where y does.)
+      const int y_up = ck_scale(abs_bits(fmaxf(wt->row[0][t.row], wt->row[1][t.row]) * dt_most), 60);
+      const float w_up = ck_power(y_up);
+      tail->y_up[t.row] = static_cast<signed char>(y_up);      // (by two threads)
       {
         // W over G: sixteen columns of scores become eight of the upper terms and eight of the lower ones
         const float4 P = *reinterpret_cast<const float4*>(tail->piece + 4 * q);
         const int r = t.lane >> 3;      // this row's piece among the four of its warp
-        const float enter = wt->enter[t.row] * sw.up;
+        const float enter = wt->enter[t.row] * w_up;
         const float p1 = r > 1 ? P.y : 1.f, p2 = r > 2 ? P.z : 1.f;
-        const f2 lead = both(enter * (r > 0 ? P.x : 1.f) * p1 * p2), up = both(sw.up);
+        const f2 lead = both(enter * (r > 0 ? P.x : 1.f) * p1 * p2), up = both(w_up);
         const uint32_t tg = lanes() + TM_G + t.half * 16;
         uint32_t v[16];
         tmem_ld_32x16(tg, v);
@@ -585,22 +622,23 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
         }
       }
       if (carried) {      // the state's share of y, to the scale of W: W x is added to it
-        const f2 f = both(wt->before[t.row] * ck_scale(cta_most(tail->most[2])).down * sw.up);
+        const f2 f = both(wt->before[t.row] * w_up);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           uint32_t v[16];
           tmem_ld_32x16(lanes() + TM_Y0 + t.half * 32 + k * 16, v);
+          const uint4 d0 = *reinterpret_cast<const uint4*>(tail->s_down + t.half * 32 + k * 16), d1 = *reinterpret_cast<const uint4*>(tail->s_down + t.half * 32 + k * 16 + 8);
+          const uint32_t d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
           tmem_ld_wait();
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
-            const float2 r = upk(mul2(f, pk(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1]))));
+            const float2 r = upk(mul2(f, mul2(ck_down(d[p]), pk(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1])))));
             v[2 * p] = __float_as_uint(r.x);
             v[2 * p + 1] = __float_as_uint(r.y);
           }
           tmem_st_32x16(lanes() + TM_Y1 + t.half * 32 + k * 16, v);
         }
       }
-      if (threadIdx.x == 0) tail->y_down = sw.down;
       tmem_st_wait();
       fence_proxy_async_smem();
       tcgen05_fence_before_sync();
@@ -626,7 +664,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_walk_kernel(const ChunkAr
       float total = 1.f;
 #pragma unroll
       for (int k = 0; k < CQ / 8; ++k) total *= tail->piece[k];
-      add_state(S, lanes() + TM_Y0 + t.half * 32, total, sv.down);
+      add_state(S, lanes() + TM_Y0 + t.half * 32, total, tail->v_down + t.half * 32);
       tcgen05_fence_before_sync();
     }
     if (t0 + CQ < length) {
@@ -710,10 +748,9 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
     if (tail->abort != 0) break;
     const StepSizes z = step_sizes(raw_next, bias, rate, true, t.lane);
     if (t.half == 0 && (t.lane & 7) == 7) tail->piece[t.row >> 3] = z.piece;
-    const uint32_t xm = warp_most(abs_bits(most_x(base + CK_X))), dm = warp_most(abs_bits(z.dt));
-    float m = 0.f;
+    bool infinite;      // in B: against the two terms of V it would be a NaN
     {
-      __half2 b2 = __float2half2_rn(0.f);      // an infinity in B, against the two terms of V, would be a NaN
+      __half2 b2 = __float2half2_rn(0.f);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const uint4 b = ck_ld(base + CK_B + t.half * CK_HALF + ck_at(t.row, k));
@@ -722,12 +759,9 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
         for (int e = 0; e < 4; ++e) b2 = __hmax2_nan(b2, __habs2(*reinterpret_cast<const __half2*>(&w[e])));
       }
       const float2 f = __half22float2(b2);
-      if (!(f.x < INFINITY && f.y < INFINITY)) m = INFINITY;
+      infinite = __any_sync(0xffffffffu, !(f.x < INFINITY && f.y < INFINITY));
     }
-    const uint32_t bm = warp_most(abs_bits(m));
-    if (t.lane == 0) { tail->most[1][t.warp] = max(xm, bm); tail->most[3][t.warp] = dm; }
     __syncthreads();
-    const uint32_t v_most = abs_bits(__uint_as_float(cta_most(tail->most[1])) * __uint_as_float(cta_most(tail->most[3])));
     float w = z.dt * z.leave, total = 1.f;
 #pragma unroll
     for (int k = 0; k < CQ / 8; ++k) {
@@ -736,11 +770,15 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
       if (k > (t.row >> 3)) w *= d;
     }
     left *= total;
-    if (odd || ck_infinite(v_most)) {
+    f2 v[16];
+    weigh(v, base + CK_X, t.row, t.half, w);
+    column_publish(tail, t, v, tail->most[1], infinite);
+    __syncthreads();
+    if (odd || cta_most(tail->most[1]) == CK_INFINITE) {
       chunk_plain<false>(ck_smem, tail, t, S, z.dt, CQ, nullptr, 0, pcols, g.N);
     } else {
-      const Scale sv = ck_scale(v_most);
-      store_v(base + CK_T, base + CK_X, t.row, t.half, w * sv.up);
+      column_scales(tail, t, tail->v_down);
+      store_terms(base + CK_T, t.row, t.half, v, tail->v_down);
       fence_proxy_async_smem();
       tcgen05_fence_before_sync();
       __syncthreads();
@@ -755,7 +793,7 @@ __global__ void __launch_bounds__(CK_THREADS, 2) chunk_states_kernel(const Chunk
       ck_wait(tail->bar + 2, finished, a.status, &tail->abort);
       finished ^= 1;
       tcgen05_fence_after_sync();
-      add_state(S, tq + t.half * 32, total, sv.down);
+      add_state(S, tq + t.half * 32, total, tail->v_down + t.half * 32);
     }
     if (t0 + CQ < sp.hi) {
       __syncthreads();

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import state_ref as ref
-from test_state_ops_gpu import select
+from test_state_ops_gpu import chunked, select, within
 
 pytestmark = pytest.mark.gpu
 TYPES = ("r16", "r32", "r64")
@@ -88,3 +88,50 @@ def test_select_masked_and_impossible_rows(mp, stream, sfx):
         with np.errstate(invalid="ignore"):
             off = np.abs(got[0].astype(np.float64) - want[0]) <= 4 * u * (1 + np.log(vocab)) + u * (vocab / 32 + 8) + u * np.abs(want[0])
         assert (off | (got[0] == want[0])).all(), (got[0], want[0])
+
+
+# ---------------------------------------------------------------------------------------------------- scan
+def check_finite_part(s, got, starts, slots, resume):
+    """Scan.check for results beyond r16's largest value too: that value stands for what lies beyond it, infinities included, on both sides (a
+    difference does not grow when both sides are cut off at the same place)."""
+    H, P, N, G = s.dims
+    most = float(np.finfo(np.float16).max)
+    (y, states), (wy, ysize, ws, ssize, ysteps, ssteps) = got, s.want(starts, slots, resume)
+    y = y[:, :s.inner].reshape(-1, H, P)[starts[0]:starts[-1]].astype(np.float64)
+    assert not np.isnan(y).any()
+    tol = ref.scan_tolerance("r16", wy, ysize, ysteps, N, True)[starts[0]:starts[-1]]
+    within(np.clip(y, -most, most), np.clip(wy[starts[0]:starts[-1]], -most, most), tol, "y")
+    within(states[slots], ws[slots], ref.scan_tolerance("r16", ws, ssize, ssteps, N, False)[slots], "states")
+
+
+@pytest.mark.parametrize("lens", [[2], [200, 90], [900, 5]])
+@pytest.mark.parametrize("shape", [(2, 64, 128, 1), (1, 80, 64, 1)])
+@pytest.mark.parametrize("what", ["x", "states", "C", "sizes", "late", "huge"])
+def test_chunks_of_values_far_apart(mp, stream, lens, shape, what):
+    """Values of one tile that lie up to 2^40 apart: each row p of a head, and each step's y, has the accuracy that it would have alone."""
+    r = np.random.default_rng(sum(lens) + sum(shape))
+    s, starts, slots, resume = chunked(r, lens, shape)
+    resume[:] = 1
+    H, P, N, G = shape
+    falling = 2.0 ** -np.round(np.linspace(0, 36, P))            # over the rows p of a head
+    rows = s.xbc.shape[0]
+    if what == "x":
+        x = s.xbc[:, :s.inner].astype(np.float64).reshape(rows, H, P) * falling * 2.0 ** 13
+        s.xbc[:, :s.inner] = x.reshape(rows, -1).astype(np.float16)
+        s.states *= (falling * 2.0 ** 13)[None, None, :, None].astype(np.float32)
+    elif what == "states":
+        s.states *= (falling * 2.0 ** 40)[None, None, :, None].astype(np.float32)
+    elif what == "C":
+        c = s.xbc[:, s.inner + s.bc:].astype(np.float64) * 2.0 ** (10 - np.arange(rows)[:, None] % 24)
+        s.xbc[:, s.inner + s.bc:] = c.astype(np.float16)
+    elif what == "sizes":
+        s.zx[:, 3:] = r.uniform(-14, 8, s.zx[:, 3:].shape).astype(np.float16)
+    elif what == "huge":      # one row of the state beside scores of next to nothing
+        s.xbc[:, s.inner:] = (s.xbc[:, s.inner:].astype(np.float64) * 2.0 ** -12).astype(np.float16)
+        s.states[:, :, 1:] = 0
+        s.states *= np.float32(2.0 ** 110)
+    else:      # nothing new in a sequence's last thirty steps, of which each leaves a fifth
+        s.zx[:, 3:], s.dt_bias[:], s.A_log[:] = 0, np.log(np.expm1(0.1)), np.log(16)
+        for lo, hi in zip(starts[:-1], starts[1:]):
+            s.xbc[max(lo, hi - 30):hi, :s.inner] = 0
+    check_finite_part(s, s.go(mp, stream, slots, resume, starts), starts, slots, resume)
