@@ -37,7 +37,11 @@ def load_weights(cfg: LMConfig, prefix: str):
 class Generator:
     """Keeps the weights, the states of `sequences` sequences (prompts times beams) and buffers for prompts of `max_rows` tokens in all.
 
-    weights: name -> array (`mamba_lm.init_weights`, `load_weights`), or a `MambaLM`, whose buffers are used as they are at each call."""
+    weights: name -> array (`mamba_lm.init_weights`, `load_weights`), or a `MambaLM`, whose buffers are used as they are at each call.
+
+    Everything runs on `stream` (a model's own, or one that the generator opens).  `prompt` and `token` take their turn behind what torch's current
+    stream holds when they are called, and that stream waits for them: tokens and logits need no synchronising there.  Work on other streams is the
+    caller's to order.  `search` waits for its results.  Call `release()` before the object goes."""
 
     def __init__(self, cfg: LMConfig, weights, sequences: int, max_rows: int, stream: Stream | None = None):
         if sequences < 1 or max_rows < 1:
@@ -100,6 +104,15 @@ class Generator:
             self._drop_graph()      # it holds the old address
             self.stream.sync()
             self.scratch = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+            torch.cuda.current_stream().synchronize()      # torch hands out memory that its own stream may still be at work on
+
+    def _behind_torch(self):
+        import torch
+        self.stream.torch_stream().wait_stream(torch.cuda.current_stream())
+
+    def _before_torch(self):
+        import torch
+        torch.cuda.current_stream().wait_stream(self.stream.torch_stream())
 
     def _upload(self, dst, values):
         a = np.ascontiguousarray(values, dtype=np.int32)
@@ -163,8 +176,9 @@ class Generator:
 
     def prompt(self, prompts, beams: int = 1):
         """Takes the prompts in; returns the r16 logits [len(prompts) * beams, vocab] behind their last tokens (a device buffer that the next
-        call overwrites).  The state of prompt i lies in sequence i * beams."""
+        call overwrites; torch's current stream waits for them).  The state of prompt i lies in sequence i * beams."""
         lens, ids = self._check(prompts, beams)
+        self._behind_torch()      # it may be reading the last logits
         n = len(prompts) * beams
         starts = np.concatenate([[0], np.cumsum(lens)])
         keep = [self._upload(self.ids, ids), self._upload(self.starts, starts), self._upload(self.slots, np.arange(len(prompts)) * beams),
@@ -175,15 +189,19 @@ class Generator:
         self._L("embedding", h, self.last_rows, self.last, n, self.cfg.d_model, rows)      # rows gathered by their numbers
         self._head(self.last, n)
         del keep
+        self._before_torch()
         return self.logits[:n]
 
     def token(self, tokens):
-        """One new token (int32, device) of each of the first len(tokens) sequences; returns their logits (see `prompt`)."""
+        """One new token (int32, device) of each of the first len(tokens) sequences; returns their logits (see `prompt`).  The tokens are read
+        behind what torch's current stream holds now."""
         import torch
         n = tokens.numel()
         if not 1 <= n <= self.sequences or tokens.dtype != torch.int32 or not tokens.is_cuda or not tokens.is_contiguous():
             raise ValueError("tokens: up to `sequences` contiguous int32 values on the device")
+        self._behind_torch()
         self._head(self._layers(tokens, n, 0), n)
+        self._before_torch()      # (so the caller may let go of the tokens too: torch reuses their memory behind this)
         return self.logits[:n]
 
     # ------------------------------------------------------------------ search
