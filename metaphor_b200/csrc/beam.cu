@@ -177,10 +177,13 @@ __host__ __device__ inline BeamScratch<A> beam_carve(void* scratch, size_t piece
 }
 template <typename A> inline size_t beam_bytes(size_t pieces) { return pieces * (2 * sizeof(double) + BM_LIST * sizeof(Entry<A>)); }
 
-// Pieces of a row: two packs for each thread of a CTA at least, eight CTAs for every SM where the rows are too few.
+// Pieces of a row: two packs for each thread of a CTA at least, eight CTAs for every SM where the rows are too few.  (148 SMs: the scratch function,
+// which goes by the same numbers, knows no device.)
+constexpr size_t BM_CTAS = 8 * 148;
+inline size_t beam_most_pieces(size_t vocab, size_t size) { return (vocab * size + 2 * 16 * BM_THREADS - 1) / (2 * 16 * BM_THREADS); }
 inline int beam_pieces(size_t rows, size_t vocab, size_t size) {
-  const size_t most = (vocab * size + 2 * 16 * BM_THREADS - 1) / (2 * 16 * BM_THREADS);
-  size_t want = 8 * 148 / rows;
+  const size_t most = beam_most_pieces(vocab, size);
+  size_t want = BM_CTAS / rows;
   if (want > most) want = most;
   return static_cast<int>(want < 1 ? 1 : want);
 }
@@ -513,7 +516,9 @@ extern "C" len_t mpBeamSelectScratchBytes(uint32_t dtype_key, len_t batch, len_t
   (void)picks;
   const size_t rows = static_cast<size_t>(batch) * beams;
   if (rows == 0) return 256;
-  const size_t size = dtype_key == MP_R16 ? 2 : dtype_key == MP_R32 ? 4 : 8, pieces = rows * beam_pieces(rows, vocab, size);
+  // No call of as many rows and tokens or fewer has more pieces in all: one a row, or not above BM_CTAS and not above the most that its rows have.
+  const size_t size = dtype_key == MP_R16 ? 2 : dtype_key == MP_R32 ? 4 : 8, most = beam_most_pieces(vocab, size);
+  const size_t cut = most != 0 && rows > BM_CTAS / most ? BM_CTAS : rows * most, pieces = cut > rows ? cut : rows;
   return static_cast<len_t>((dtype_key == MP_R64 ? beam_bytes<double>(pieces) : beam_bytes<float>(pieces)) + 256);
 }
 

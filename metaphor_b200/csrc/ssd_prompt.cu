@@ -280,19 +280,21 @@ struct Cut { int lanes, splits, steps; size_t ids; };      // lanes of a row; CT
 // are not eight CTAs for each of 148 SMs all the same (three fit at a time): a range's state is made twice.  Measured, r32, whole and in ranges: one
 // sequence of 256 steps and 24 heads 28 and 46 us, of 512 steps 52 and 44, with 4 heads 51 and 22 (25 with ranges of 64 steps at least).  Rows get more lanes where a head is small, or where there are fewer than two CTAs for an SM (12 sequences of up to 300
 // steps: 95 us, with one CTA for an SM 143, with four 105).
+// (148 SMs: the scratch function, which goes by the same numbers, knows no device.)
+constexpr size_t RC_SMS = 148, RC_CTAS = 8 * RC_SMS, RC_LONG = 320, RC_RANGE = 32;
 Cut recurrence_cut(size_t nseq, size_t rows, size_t heads, size_t headdim, int held, int least, int most) {
   Cut c{least, 0, 0, nseq};
   auto rows_of = [&] { return static_cast<size_t>(held) * (128 / c.lanes); };
   auto splits = [&] { return (headdim + rows_of() - 1) / rows_of(); };
   while (c.lanes < most && 2 * headdim <= rows_of()) c.lanes <<= 1;
   const size_t units = heads * splits(), longest = 2 * rows / nseq < rows ? 2 * rows / nseq : rows;      // (a guess)
-  if (nseq * units < 8 * 148 && longest > 320) {
-    const size_t want = 8 * 148 / units + 1;
+  if (nseq * units < RC_CTAS && longest > RC_LONG) {
+    const size_t want = RC_CTAS / units + 1;
     size_t range = ((rows + want - 1) / want + 15) / 16 * 16;
-    if (range < 32) range = 32;
+    if (range < RC_RANGE) range = RC_RANGE;
     if (range < rows) { c.steps = static_cast<int>(range); c.ids = rows / range + nseq; }
   }
-  while (c.lanes < most && c.ids * heads * splits() < 2 * 148) c.lanes <<= 1;
+  while (c.lanes < most && c.ids * heads * splits() < 2 * RC_SMS) c.lanes <<= 1;
   c.splits = static_cast<int>(splits());
   return c;
 }
@@ -329,11 +331,20 @@ auto by_columns(size_t dstate, F what) {
 }
 template <typename T> constexpr int recurrence_held = RecurrenceSizes<T, 32, 8>::PV;
 
+// Enough for every call of as many sequences and rows or fewer: those that are cut have fewer than RC_CTAS units in all (a head's CTAs do not depend on
+// either), ranges of RC_RANGE steps or more, no more of them than `recurrence_cut` wants, and a sequence above RC_LONG by its guess.
 template <typename T>
 size_t recurrence_scratch(size_t nseq, size_t rows, size_t heads, size_t headdim, size_t dstate) {
   if (nseq == 0 || heads == 0 || headdim == 0 || dstate == 0 || dstate > 256) return 256;
-  const Cut c = by_columns(dstate, [&](auto, auto least, auto most) { return recurrence_cut(nseq, rows, heads, headdim, recurrence_held<T>, least.value, most.value); });
-  return c.steps == 0 ? 256 : c.ids * heads * (headdim * dstate + 1) * sizeof(typename Acc<T>::type) + 256;
+  const size_t units = by_columns(dstate, [&](auto, auto least, auto most) {
+    return heads * static_cast<size_t>(recurrence_cut(RC_CTAS, 0, heads, headdim, recurrence_held<T>, least.value, most.value).splits);
+  });
+  size_t sequences = (RC_CTAS - 1) / units, ranges = RC_CTAS / units + 1;
+  if (sequences > nseq) sequences = nseq;
+  if (sequences > 2 && sequences > 2 * rows / RC_LONG) sequences = 2 * rows / RC_LONG;
+  if (ranges > rows / RC_RANGE) ranges = rows / RC_RANGE;
+  if (sequences == 0 || rows <= RC_LONG) return 256;
+  return (ranges + sequences) * heads * (headdim * dstate + 1) * sizeof(typename Acc<T>::type) + 256;
 }
 
 template <typename T>

@@ -864,10 +864,12 @@ __global__ void __launch_bounds__(256) chunk_carry_kernel(const ChunkArgs a) {
 }
 
 // Steps of a range, 0 for whole sequences.  The host knows how many sequences and rows there are, not how long each is.  Where the sequences'
-// heads fill the SMs, whole ones: ranges make every state twice.  Otherwise two CTAs for each of 148 SMs, of two chunks at least.
+// heads fill the SMs, whole ones: ranges make every state twice.  Otherwise two CTAs for each of 148 SMs (the scratch function, which goes by the same
+// numbers, knows no device), of two chunks at least.
+constexpr size_t CK_SMS = 148;
 int chunk_range(size_t nseq, size_t rows, size_t units) {
-  if (nseq * units >= 148) return 0;
-  const size_t want = 2 * 148 / units;
+  if (nseq * units >= CK_SMS) return 0;
+  const size_t want = 2 * CK_SMS / units;
   size_t range = ((rows + want - 1) / want + CQ - 1) / CQ * CQ;
   if (range < 2 * CQ) range = 2 * CQ;
   return range >= rows ? 0 : static_cast<int>(range);
@@ -884,8 +886,12 @@ bool mp_ssd_prompt_chunks_take(const PromptArgs& g) {
 size_t mp_ssd_prompt_chunks_scratch(size_t nseq, size_t rows, size_t heads, size_t headdim, size_t dstate) {
   const size_t units = heads * ((headdim + CP - 1) / CP);
   if (units == 0 || nseq == 0 || dstate > CN) return 256;
-  const int range = chunk_range(nseq, rows, units);
-  return range == 0 ? 256 : chunk_ids(nseq, rows, range) * units * (CP * CN + 1) * sizeof(float) + 256;
+  // Enough for every call of as many sequences and rows or fewer: those that are cut have fewer than CK_SMS units in all, ranges of two chunks or more,
+  // and no more of them than `chunk_range` wants.
+  const size_t sequences = nseq < (CK_SMS - 1) / units ? nseq : (CK_SMS - 1) / units;
+  if (sequences == 0 || rows <= 2 * CQ) return 256;
+  const size_t want = 2 * CK_SMS / units, ranges = want < rows / (2 * CQ) ? want : rows / (2 * CQ);
+  return (ranges + sequences) * units * (CP * CN + 1) * sizeof(float) + 256;
 }
 
 void mp_ssd_prompt_chunks(const PromptArgs& g, void* scratch, StreamContext ctx) {
