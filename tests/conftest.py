@@ -40,6 +40,21 @@ def pytest_collection_modifyitems(config, items):
             item.add_marker(skip)
 
 
+@pytest.fixture(scope="module", autouse=True)
+def refused_calls_see_no_device(request):
+    """Tests of refusals call launchers with made-up addresses in processes of their own.  A refusal that went missing must end there, not on a GPU."""
+    if not request.module.__name__.endswith("refusals"):
+        yield
+        return
+    before = os.environ.get("CUDA_VISIBLE_DEVICES")
+    os.environ["CUDA_VISIBLE_DEVICES"] = ""
+    yield
+    if before is None:
+        del os.environ["CUDA_VISIBLE_DEVICES"]
+    else:
+        os.environ["CUDA_VISIBLE_DEVICES"] = before
+
+
 @pytest.fixture(scope="session")
 def mp():
     import metaphor_b200
