@@ -490,6 +490,7 @@ void beam_select_impl(const void* logits, len_t logits_pitch, const void* scores
   if (batch == 0) return;
   if (scratch == nullptr) MP_FATAL("beam_select: scratch must not be NULL (mpBeamSelectScratchBytes)");
   if (reinterpret_cast<uintptr_t>(scratch) % 8 != 0) MP_FATAL("beam_select: scratch must be 8-byte aligned");
+  if (batch > 0x7fffffffull) MP_FATAL("beam_select: %lu searches are too many for one launch", batch);
   const size_t rows = static_cast<size_t>(batch) * beams;
   const int pieces = beam_pieces(rows, vocab, sizeof(T));
   if (rows * pieces > 0x7fffffffull) MP_FATAL("beam_select: %lu searches are too many for one launch", batch);

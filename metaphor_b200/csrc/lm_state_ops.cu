@@ -362,8 +362,6 @@ __global__ void reorder_kernel(unsigned char* __restrict__ states, const int* __
 }
 
 // ------------------------------- launch bodies ------------------------------
-bool fits(len_t v) { return v <= 0x7fffffffull; }
-
 template <typename T, int V>
 void conv_prompt_run(const T* x, size_t xp, const T* w, const T* bias, T* states, T* y, size_t yp, const Sequences& q, int channels, int width, StreamContext ctx) {
   const int cols = (channels + V * CS_TX - 1) / (V * CS_TX);
@@ -386,7 +384,7 @@ template <typename T>
 void conv_check(const char* name, len_t rows, len_t nslots, len_t channels, len_t width, len_t x_pitch, len_t y_pitch) {
   if (width < 2 || width > 4) MP_FATAL("%s: width %lu is not 2, 3 or 4", name, width);
   if (x_pitch < channels || y_pitch < channels) MP_FATAL("%s: a row pitch is below the %lu channels", name, channels);
-  if (!fits(rows) || !fits(nslots) || !fits(channels * width)) MP_FATAL("%s: rows, slots and channels are counted in 31 bits", name);
+  if (!fits(rows) || !fits(nslots) || !fits(channels, width)) MP_FATAL("%s: rows, slots and channels are counted in 31 bits", name);
 }
 
 template <typename T>
@@ -446,9 +444,9 @@ void ssd_scan_token_impl(const void* x, len_t x_pitch, const void* dt_raw, len_t
                          len_t headdim, len_t dstate, len_t ngroups, StreamContext ctx) {
   using A = typename Acc<T>::type;
   if (ngroups == 0 || heads % ngroups != 0) MP_FATAL("ssd_scan_token: heads %lu not divisible by groups %lu", heads, ngroups);
-  if (x_pitch < heads * headdim || y_pitch < heads * headdim || bc_pitch < ngroups * dstate || dt_pitch < heads) MP_FATAL("ssd_scan_token: a row pitch is below its columns");
-  if (!fits(rows) || !fits(nslots) || !fits(heads * headdim) || !fits(headdim * dstate) || dstate > 1ull << 30)
+  if (!fits(rows) || !fits(nslots) || !fits(heads, headdim) || !fits(headdim, dstate) || !fits(ngroups, dstate) || headdim > SEQ_HEADDIM || dstate > 1ull << 30)
     MP_FATAL("ssd_scan_token: rows, slots and sizes are counted in 31 bits");
+  if (x_pitch < heads * headdim || y_pitch < heads * headdim || bc_pitch < ngroups * dstate || dt_pitch < heads) MP_FATAL("ssd_scan_token: a row pitch is below its columns");
   if (rows == 0 || heads == 0 || headdim == 0) return;
   if (dstate == 0) MP_FATAL("ssd_scan_token: no state");
   const int P = static_cast<int>(headdim), N = static_cast<int>(dstate);
@@ -514,8 +512,8 @@ void reorder_states_impl(void* states, const void* slots, const void* parents, l
   if (beams > 64) MP_FATAL("reorder_states: %lu beams (64 at most)", beams);
   if (batch > 65535 || !fits(nslots) || !fits(layers)) MP_FATAL("reorder_states: searches are counted in 16 bits, slots and layers in 31");
   if (layers == 0 || batch == 0 || beams == 0 || row == 0) return;
+  if (row > (0x7fffffffull * 32 + 31) / sizeof(T)) MP_FATAL("reorder_states: rows of %lu elements are too long", row);
   const size_t bytes = static_cast<size_t>(row) * sizeof(T);
-  if (bytes / 2 / 16 > 0x7fffffffull) MP_FATAL("reorder_states: rows of %lu elements are too long", row);
   const int *sl = static_cast<const int*>(slots), *pa = static_cast<const int*>(parents);
   const size_t align = reinterpret_cast<uintptr_t>(states) | bytes;
   const long long L = static_cast<long long>(layers), b = static_cast<long long>(batch), n = static_cast<long long>(nslots), rb = static_cast<long long>(bytes);

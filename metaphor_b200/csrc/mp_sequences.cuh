@@ -4,6 +4,12 @@
 
 #include "mp_async.cuh"
 
+// Sizes are counted in 31 bits, and so are products of two (each asked first: the product of larger ones may wrap round).
+inline bool fits(len_t v) { return v <= 0x7fffffffull; }
+inline bool fits(len_t a, len_t b) { return fits(a) && fits(b) && fits(a * b); }
+// A head's rows p: the kernels round them up to whole tiles.
+constexpr len_t SEQ_HEADDIM = 1ull << 30;
+
 // Sequence i has the rows starts[i] .. starts[i + 1] of the packed buffers and row slots[i] of the state buffer; it goes on from that state
 // where resume[i] is not zero.  The three arrays lie on the device: nothing about them is known when a launch is made, so every use is clamped
 // to the buffers that the launch names.

@@ -370,16 +370,15 @@ void recurrence(const PromptArgs& g, void* scratch, StreamContext ctx) {
   });
 }
 
-bool fits(len_t v) { return v <= 0x7fffffffull; }
-
 template <typename T>
 void ssd_scan_prompt_impl(const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* Bm,
                           const void* Cm, len_t bc_pitch, void* states, const void* slots, const void* resume, const void* starts, void* y, len_t y_pitch,
                           void* scratch, len_t nseq, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext ctx) {
   if (ngroups == 0 || heads % ngroups != 0) MP_FATAL("ssd_scan_prompt: heads %lu not divisible by groups %lu", heads, ngroups);
-  if (x_pitch < heads * headdim || y_pitch < heads * headdim || bc_pitch < ngroups * dstate || dt_pitch < heads) MP_FATAL("ssd_scan_prompt: a row pitch is below its columns");
-  if (!fits(nseq) || !fits(rows) || !fits(nslots) || !fits(heads * headdim)) MP_FATAL("ssd_scan_prompt: sequences, rows, slots and columns are counted in 31 bits");
   if (dstate == 0 || dstate > 256) MP_FATAL("ssd_scan_prompt: state size %lu (1 to 256)", dstate);
+  if (!fits(nseq) || !fits(rows) || !fits(nslots) || !fits(heads, headdim) || !fits(ngroups, dstate) || headdim > SEQ_HEADDIM)
+    MP_FATAL("ssd_scan_prompt: sequences, rows, slots and columns are counted in 31 bits");
+  if (x_pitch < heads * headdim || y_pitch < heads * headdim || bc_pitch < ngroups * dstate || dt_pitch < heads) MP_FATAL("ssd_scan_prompt: a row pitch is below its columns");
   if (nseq == 0 || heads == 0 || headdim == 0) return;
   PromptArgs g{x, dt_raw, dt_bias, A_log, Bm, Cm, states, y, x_pitch, dt_pitch, bc_pitch, y_pitch,
                Sequences{static_cast<const int*>(starts), static_cast<const int*>(slots), static_cast<const int*>(resume), static_cast<int>(nseq),
