@@ -291,10 +291,14 @@ MP_DECL3(causal_conv1d_silu_token, const void* x, len_t x_pitch, const void* w, 
 /* The SSD scan from the projection's raw outputs (launch_ssd_scan_raw) that begins with each sequence's state:
  *   dt = softplus(dt_raw + dt_bias[h]),  S_t = exp(-dt_t exp(A_log[h])) S_{t-1} + dt_t x_t (x) B_t,  y_t = S_t C_t.
  * x, y: rows of heads * headdim elements, B, C: rows of ngroups * dstate, dt_raw: rows of heads, all of T with row pitches of
- * their own (B and C share one); dt_bias, A_log: acc [heads]; states: acc [nslots, heads, headdim, dstate].  dstate is 256
- * at most in the prompt form; sizes and heads * headdim are counted in 31 bits, headdim and dstate are 2^30 at most.  Prompt scratch: mpSsdScanPromptScratchBytes(...) bytes owned by the caller, 16-byte aligned, which are
- * enough for every call of the same type, heads, headdim and dstate with as many sequences and rows or fewer; NULL: long sequences are
- * not cut into ranges that run side by side. */
+ * their own (B and C share one); dt_bias, A_log: acc [heads]; states: acc [nslots, heads, headdim, dstate].  Sizes and their products
+ * are counted in 31 bits, headdim and dstate are 2^30 at most, dstate 256 in the prompt form.
+ * Prompt scratch: mpSsdScanPromptScratchBytes(...) bytes owned by the caller, 16-byte aligned, which are enough for every call of the
+ * same type, heads, headdim and dstate with as many sequences and rows or fewer; NULL: long sequences are not cut into ranges that run
+ * side by side.
+ * r16 prompts whose headdim, dstate and pitches (but dt_raw's) are multiples of 8, with 16-byte aligned pointers and a dstate of 128 at
+ * most, go through the tensor cores in chunks of 128 steps.  What a step adds to row p of a head's state is then off by up to 2^-22 of itself
+ * or 2^-39 of the largest such value of that row in the chunk, whichever is more; other prompts go step by step in the accumulator type. */
 MP_DECL3(ssd_scan_prompt, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, const void* resume, const void* starts, void* y, len_t y_pitch, void* scratch, len_t nseq, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
 MP_DECL3(ssd_scan_token, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, void* y, len_t y_pitch, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
 MP_EXTERN_C len_t mpSsdScanPromptScratchBytes(uint32_t dtype_key, len_t nseq, len_t rows, len_t heads, len_t headdim, len_t dstate, len_t ngroups);

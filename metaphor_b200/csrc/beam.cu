@@ -5,10 +5,11 @@
 // 32 best logits; the second adds the pieces up, forms the scores in r64 and merges the beams.
 //
 // The best of a piece.  While it streams by, a thread keeps its own maximum only.  Sorted inside a warp, the maxima give a bound that at least
-// `picks` values reach: the least of the warps' values at place ceil(picks / warps).  Threads whose maximum reaches it (some tens of 256) look
-// at their values again, which the L2 still has, and put those that reach it on a list in shared memory; one warp sorts it, 32 at a time, by
-// bitonic stages.  So what is done for every value is one exponential, its sum and a comparison.  Where the list would overflow (rows of few
-// different values), every value is offered to a warp's list of 32 in turn instead.
+// `picks` values reach: the least of the warps' values at place ceil(picks / warps).  Threads whose maximum reaches it (some tens of 128) look
+// again at the one or two packs that they remember for it, or at all of theirs where a third one reaches it too, which the L2 still has, and put
+// what reaches it on a list in shared memory; the warps sort it, 32 at a time, by bitonic stages and merge what they have.  So what is done for
+// every value is one exponential, its sum and a comparison.  Where the list would overflow (rows of few different values), every value is offered
+// to a warp's list of 32 in turn instead.
 // Measured (r16, 50280 logits a row): 64 searches of 8 beams and 16 picks 27.4 us (rows 19, beams 7; the bytes take 7.9), one of 4 beams and 4
 // picks 10.7 us.  Rows come at 4 TB/s, one exponential a value keeps the special-function unit busy for 4.9 us; beside them stand about 8 us of
 // latency in a row's own steps (maxima, bound, second look, list) and the merge's sorts, shuffle behind shuffle.  Inserting every candidate into a

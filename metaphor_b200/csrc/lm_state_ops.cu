@@ -52,7 +52,7 @@ __device__ __forceinline__ StVec<T, V> silu_vec(const typename Acc<T>::type (&v)
 // Convolution over packed prompts.  A thread has V channels and a run of `run` rows, which it walks with the last W - 1 inputs in registers.
 // Rows that reach into the kept state (the first W - 1 of a sequence) belong to the thread that has the sequence's first row, even behind its
 // run's end, and that thread writes the new state too, from inputs that it fetches again: so nobody else reads what it overwrites.
-// Measured (r16, 16 prompts of 8264 rows in all, 1792 channels): 17.5 us, 3.0 TB/s.  The special-function unit, which gives 16 of a value's two
+// Measured (r16, 16 prompts of 7375 rows in all, 1792 channels): 17.5 us, 3.0 TB/s.  The special-function unit, which gives 16 of a value's two
 // results a clock, is busy for 6.6 us of it; the rest is the way to the first inputs (sequence, state, taps) and too few warps to hide it.
 // ---------------------------------------------------------------------------
 constexpr int CS_TX = 32, CS_TY = 4, CS_U = 8;

@@ -277,10 +277,11 @@ __global__ void __launch_bounds__(256) recurrence_carry_kernel(const PromptArgs 
 // How a call is cut up.  The host knows how many sequences and rows there are, not how long each is.
 struct Cut { int lanes, splits, steps; size_t ids; };      // lanes of a row; CTAs of a head; steps of a range (0: whole sequences); ranges or sequences
 // `least`, `most`: lanes of a row; `held`: rows p of a lane.  Ranges of 32 steps or more where a sequence may be longer than 320 steps and there
-// are not eight CTAs for each of 148 SMs all the same (three fit at a time): a range's state is made twice.  Measured, r32, whole and in ranges: one
-// sequence of 256 steps and 24 heads 28 and 46 us, of 512 steps 52 and 44, with 4 heads 51 and 22 (25 with ranges of 64 steps at least).  Rows get more lanes where a head is small, or where there are fewer than two CTAs for an SM (12 sequences of up to 300
-// steps: 95 us, with one CTA for an SM 143, with four 105).
-// (148 SMs: the scratch function, which goes by the same numbers, knows no device.)
+// are not eight CTAs for each of 148 SMs all the same (three fit at a time, two of 256 columns in fp32): a range's state is made twice.  Measured,
+// r32, whole and in ranges: one sequence of 256 steps and 24 heads 28 and 46 us, of 512 steps 52 and 44, with 4 heads 51 and 22 (25 with ranges of
+// 64 steps at least); five of up to 333 steps and 8 heads 39 and 41, which the guess at the longest cannot tell from one long among short ones.
+// Rows get more lanes where a head is small, or where there are fewer than two CTAs for an SM (12 sequences of up to 300 steps: 95 us, with one CTA
+// for an SM 143, with four 105).  (148 SMs: the scratch function, which goes by the same numbers, knows no device.)
 constexpr size_t RC_SMS = 148, RC_CTAS = 8 * RC_SMS, RC_LONG = 320, RC_RANGE = 32;
 Cut recurrence_cut(size_t nseq, size_t rows, size_t heads, size_t headdim, int held, int least, int most) {
   Cut c{least, 0, 0, nseq};
