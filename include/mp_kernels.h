@@ -298,7 +298,7 @@ MP_DECL3(causal_conv1d_silu_token, const void* x, len_t x_pitch, const void* w, 
  * side by side.
  * r16 prompts whose headdim, dstate and pitches (but dt_raw's) are multiples of 8, with 16-byte aligned pointers and a dstate of 128 at
  * most, go through the tensor cores in chunks of 128 steps.  What a step adds to row p of a head's state is then off by up to 2^-22 of itself
- * or 2^-39 of the largest such value of that row in the chunk, whichever is more; other prompts go step by step in the accumulator type. */
+ * or 2^-38 of the largest such value of that row in the chunk, whichever is more; other prompts go step by step in the accumulator type. */
 MP_DECL3(ssd_scan_prompt, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, const void* resume, const void* starts, void* y, len_t y_pitch, void* scratch, len_t nseq, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
 MP_DECL3(ssd_scan_token, const void* x, len_t x_pitch, const void* dt_raw, len_t dt_pitch, const void* dt_bias, const void* A_log, const void* B, const void* C, len_t bc_pitch, void* states, const void* slots, void* y, len_t y_pitch, len_t rows, len_t nslots, len_t heads, len_t headdim, len_t dstate, len_t ngroups, StreamContext stream)
 MP_EXTERN_C len_t mpSsdScanPromptScratchBytes(uint32_t dtype_key, len_t nseq, len_t rows, len_t heads, len_t headdim, len_t dstate, len_t ngroups);
